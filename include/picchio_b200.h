@@ -297,6 +297,127 @@ pc_status pc_qt_check(pc_qt *w, void *stream);
 pc_status pc_qt_dequant(pc_qt *w, float *out_dev, void *stream);
 void pc_qt_free(pc_qt *w);
 
+/* ---- paged KV cache: tables, store, attention ------------------------------ */
+
+/* Operators of a serving step whose KV cache is cut into pages that requests
+ * take and give back, for programs that keep their own caches.  (pc_ctx keeps
+ * one fixed-length slot per sequence, as the reference does; the reference
+ * has no paged cache.)  They work on device tensors of any producer, run on
+ * the `stream` they are given, return without waiting for it and allocate
+ * nothing, so they can be captured into a CUDA graph.  A request's tokens
+ * stand at positions 0, 1, ...; position p is in page page_table[request][p /
+ * page_size], row p % page_size.  One layer's cache is one pc_kv_pages; the
+ * tables serve every layer. */
+
+/* Element types of K, V, q and out. */
+enum { PC_DT_F32 = 0, PC_DT_F16 = 1, PC_DT_BF16 = 2 };
+
+/* One layer's pages.  Element (page, row, KV head, i) of K is at k_dev +
+ * page * k_stride[0] + row * k_stride[1] + head * k_stride[2] + i, of V
+ * likewise; strides count elements.  Pointers and strides are multiples of 16
+ * bytes. */
+typedef struct {
+    void *k_dev, *v_dev;
+    int64_t k_stride[3], v_stride[3];
+    int dtype;      /* PC_DT_* */
+    int n_pages;
+    int page_size;  /* positions per page: a multiple of 8 */
+    int n_kv_heads;
+    int head_dim;   /* a multiple of 8, at most 128 */
+} pc_kv_pages;
+
+/* The tables of one serving step, from the requests' lengths.
+ *  in   kv_len[b]   positions request b holds (below 0 counts as 0)
+ *       new_len[b]  positions it adds in this step; below 0: it has ended
+ *       n_free      free page ids in free_pages[0 .. n_free), the next one last
+ *  in/out  page_table[b][0 .. max_pages): the first ceil(kv_len / page_size)
+ *       entries are request b's pages; those of the pages it gets are written
+ *       free_pages[0 .. free_cap): the pages of ended requests are put on top,
+ *       in request order, before any is handed out
+ *  out  kv_end[b]   kv_len + new_len of a served request, kv_len of one that
+ *       is not served, 0 of an ended one
+ *       cu_new[0 .. n_requests]: prefix sums of the served new positions;
+ *       served[b]   1: request b got what it needs in this step
+ *       n_free_out  free pages left
+ *       pos[t], slot[t], t < n_tokens: position of the step's row t in its
+ *       request and its slot page * page_size + row; -1 from row
+ *       cu_new[n_requests] on
+ * Request b is not served if its new length exceeds max_pages pages, or if
+ * it needs pages and the needs of requests 0 .. b exceed the free ones, or if
+ * it adds positions and those of requests 0 .. b exceed n_tokens (sums over
+ * all requests that fit their table).  The inputs other than page_table and
+ * free_pages are not written: a call repeated with the same inputs gives the
+ * same outputs, and the next step's inputs are kv_end and n_free_out.  kv_end
+ * and n_free_out must not overlap the inputs. */
+typedef struct {
+    int n_requests, max_pages, page_size, n_tokens, free_cap;
+    const int *kv_len_dev, *new_len_dev, *n_free_dev;
+    int *page_table_dev, *free_pages_dev;
+    int *kv_end_dev, *cu_new_dev, *served_dev, *n_free_out_dev, *pos_dev;
+    int64_t *slot_dev;
+} pc_kv_step;
+pc_status pc_kv_tables(int device, const pc_kv_step *step, void *stream);
+
+/* Writes n rows of new K and V (src_dtype, [n][n_kv_heads][head_dim] with
+ * strides {row, head} in elements; pointers and strides multiples of 16
+ * bytes) to their slots, rounded once to the cache's type.  Rows whose slot
+ * is outside [0, n_pages * page_size) are skipped; no slot may occur twice. */
+pc_status pc_kv_store(int device, const pc_kv_pages *kv, const void *k_dev, const int64_t *k_stride,
+                      const void *v_dev, const int64_t *v_stride, int src_dtype, const int64_t *slot_dev, int n,
+                      void *stream);
+
+/* Attention of packed rows: rows cu_new[b] .. cu_new[b + 1] of q and out are
+ * request b's.  Query head h reads KV head h / (n_heads / n_kv_heads).  The
+ * row at position p sees keys max(0, p - window + 1) .. p (all up to p when
+ * window is 0):
+ *   out = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink_h - m)),
+ *   s_j = scale * q . k_j, m the largest s_j or sink_h
+ * (without sinks, no sink term).  Keys a row does not see have no part in
+ * it, whatever their K and V hold (stale pages, NaN).  A row that sees no key
+ * gives zeros.  Sums and softmax statistics are fp32; for 16-bit types the
+ * softmax weights are rounded to that type before they meet V. */
+typedef struct {
+    const void *q_dev;     /* [n_rows][n_heads][head_dim] */
+    int64_t q_stride[2];   /* elements: row, head */
+    void *out_dev;
+    int64_t out_stride[2];
+    int dtype;             /* PC_DT_*, of q, out, K and V */
+    int n_heads, n_kv_heads;
+    int head_dim;          /* a multiple of 8, at most 128 */
+    int n_rows;            /* rows of q and out; those past cu_new[n_requests] are left alone */
+    int n_requests;
+    const int *cu_new_dev; /* [n_requests + 1], from 0, ascending */
+    const float *sinks_dev; /* [n_heads] or NULL */
+    int window;            /* positions a row sees, itself included; 0: all */
+    float scale;           /* 1 / sqrt(head_dim) as a rule */
+} pc_attn_call;
+
+/* Workspace of the attention calls on one GPU: what the thread blocks that
+ * share a row's keys leave for one another (a few tens of MB).  Calls on one
+ * handle run one after another: use one handle per stream. */
+typedef struct pc_attn pc_attn;
+pc_status pc_attn_create(int device, pc_attn **out);
+void pc_attn_free(pc_attn *a);
+
+/* Attention of each request's new rows over its pages.  kv_len[b] positions
+ * of request b are in the cache, its new rows (stored before the call) among
+ * them as the last: row i stands at position kv_len - (cu_new[b + 1] -
+ * cu_new[b]) + i.  kv_len beyond max_pages pages is cut to them; a page id
+ * outside the cache reads as zeros. */
+pc_status pc_attn_paged(pc_attn *a, const pc_attn_call *call, const pc_kv_pages *kv, const int *page_table_dev,
+                        int max_pages, const int *kv_len_dev, void *stream);
+
+/* Attention over whole prompts: k and v are packed as q is, [n_rows]
+ * [n_kv_heads][head_dim] with strides {row, head} in elements, and row i of a
+ * request stands at position i. */
+pc_status pc_attn_packed(pc_attn *a, const pc_attn_call *call, const void *k_dev, const int64_t *k_stride,
+                         const void *v_dev, const int64_t *v_stride, void *stream);
+
+/* Waits for `stream`, then reports (PC_ERR_TIMEOUT) and clears a device-side
+ * failure of earlier calls on the handle: a bounded wait of an attention
+ * kernel giving up. */
+pc_status pc_attn_check(pc_attn *a, void *stream);
+
 /* ---- expert parallelism -------------------------------------------------- */
 
 /* Writes a fresh 128-byte ncclUniqueId (rank 0 calls this and shares it). */

@@ -9,3 +9,4 @@ from .api import (  # noqa: F401
     PicchioError, Model, ModelConfig, QT, nccl_unique_id, lib, LIB_PATH,
     FMT_F32, FMT_INT8, FMT_INT4, FMT_MXFP4,
 )
+from .paged import Attention, StepTables, kv_store, kv_tables  # noqa: F401

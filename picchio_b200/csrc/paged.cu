@@ -1,0 +1,248 @@
+// paged.cu - the C entry points of the paged KV cache operators: checks of
+// their arguments, the attention workspace, and the choice of a kernel.
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cstring>
+#include <string>
+
+#include "context.h"
+#include "paged.h"
+
+struct pc_attn {
+    int dev = 0, nsm = 148, max_smem = 0;
+    float *part = nullptr;
+    unsigned *ticket = nullptr;
+    int *err = nullptr;
+};
+
+namespace {
+
+using namespace pc;
+
+// The device of a call, and the caller's again when it returns.
+struct OnDevice {
+    int old = -1;
+    cudaError_t e;
+    explicit OnDevice(int dev) {
+        e = cudaGetDevice(&old);
+        if (e == cudaSuccess && old != dev) e = cudaSetDevice(dev);
+        else old = -1;
+    }
+    ~OnDevice() {
+        if (old >= 0) cudaSetDevice(old);
+    }
+};
+
+int dt_size(int dt) { return dt == PC_DT_F32 ? 4 : 2; }
+bool dt_ok(int dt) { return dt == PC_DT_F32 || dt == PC_DT_F16 || dt == PC_DT_BF16; }
+
+// Rows start on 16-byte boundaries (16-byte loads, tensor maps).
+bool aligned(const void *p, const int64_t *s, int n, int esize) {
+    if ((uintptr_t)p % 16) return false;
+    for (int i = 0; i < n; ++i)
+        if (s[i] < 0 || (s[i] * esize) % 16) return false;
+    return true;
+}
+
+pc_status check_pages(const pc_kv_pages *kv) {
+    if (!kv || !kv->k_dev || !kv->v_dev || kv->n_pages < 1 || kv->n_kv_heads < 1)
+        return fail(PC_ERR_INVALID_ARG, "bad pc_kv_pages");
+    if (!dt_ok(kv->dtype)) return fail(PC_ERR_FORMAT, "cache type must be PC_DT_F32, PC_DT_F16 or PC_DT_BF16");
+    if (kv->head_dim < 8 || kv->head_dim > 128 || kv->head_dim % 8)
+        return fail(PC_ERR_FORMAT, "head_dim must be a multiple of 8, at most 128");
+    if (kv->page_size < 8 || kv->page_size % 8 || kv->page_size > (1 << 16))
+        return fail(PC_ERR_FORMAT, "page_size must be a multiple of 8, at most 65536");
+    const int es = dt_size(kv->dtype);
+    if (!aligned(kv->k_dev, kv->k_stride, 3, es) || !aligned(kv->v_dev, kv->v_stride, 3, es))
+        return fail(PC_ERR_FORMAT, "K and V pages need 16-byte aligned pointers and strides");
+    return PC_OK;
+}
+
+pc_status check_call(const pc_attn_call *c) {
+    if (!c || c->n_rows < 0 || c->n_requests < 0 || c->n_heads < 1 || c->n_kv_heads < 1 || c->window < 0)
+        return fail(PC_ERR_INVALID_ARG, "bad pc_attn_call");
+    if (c->n_heads % c->n_kv_heads) return fail(PC_ERR_INVALID_ARG, "n_heads must be a multiple of n_kv_heads");
+    if (c->n_heads / c->n_kv_heads > 128) return fail(PC_ERR_FORMAT, "at most 128 query heads per KV head");
+    if (!dt_ok(c->dtype)) return fail(PC_ERR_FORMAT, "type must be PC_DT_F32, PC_DT_F16 or PC_DT_BF16");
+    if (c->head_dim < 8 || c->head_dim > 128 || c->head_dim % 8)
+        return fail(PC_ERR_FORMAT, "head_dim must be a multiple of 8, at most 128");
+    if (c->n_rows > (1 << 24) / (c->n_heads / c->n_kv_heads) * 8 || c->n_requests > (1 << 24))
+        return fail(PC_ERR_RANGE, "too many rows or requests");
+    if (c->n_rows == 0 || c->n_requests == 0) return PC_OK;
+    if (!c->q_dev || !c->out_dev || !c->cu_new_dev) return fail(PC_ERR_INVALID_ARG, "null tensor");
+    const int es = dt_size(c->dtype);
+    if (!aligned(c->q_dev, c->q_stride, 2, es) || !aligned(c->out_dev, c->out_stride, 2, es))
+        return fail(PC_ERR_FORMAT, "q and out need 16-byte aligned pointers and strides");
+    return PC_OK;
+}
+
+AttnOp op_of(const pc_attn *a, const pc_attn_call *c) {
+    AttnOp o;
+    memset(&o, 0, sizeof o);
+    o.q = c->q_dev;
+    o.out = c->out_dev;
+    for (int i = 0; i < 2; ++i) {
+        o.qs[i] = c->q_stride[i];
+        o.os[i] = c->out_stride[i];
+    }
+    o.cu = c->cu_new_dev;
+    o.sinks = c->sinks_dev;
+    o.B = c->n_requests;
+    o.T = c->n_rows;
+    o.H = c->n_heads;
+    o.KVH = c->n_kv_heads;
+    o.G = c->n_heads / c->n_kv_heads;
+    o.D = c->head_dim;
+    o.window = c->window;
+    o.scale = c->scale;
+    o.min_q = 1;
+    o.max_q = INT_MAX;
+    o.part = a->part;
+    o.ticket = a->ticket;
+    o.err = a->err;
+    return o;
+}
+
+pc_status run_attention(pc_attn *a, const AttnOp &o, int dtype, cudaStream_t st) {
+    PC_CU(launch_attn_simt(o, dtype, a->nsm, st));
+    return PC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+pc_status pc_kv_tables(int device, const pc_kv_step *s, void *stream) {
+    if (!s || s->n_requests < 1 || s->max_pages < 1 || s->n_tokens < 0 || s->free_cap < 0 || !s->kv_len_dev ||
+        !s->new_len_dev || !s->n_free_dev || !s->page_table_dev || !s->kv_end_dev || !s->cu_new_dev ||
+        !s->served_dev || !s->n_free_out_dev || (s->free_cap > 0 && !s->free_pages_dev) ||
+        (s->n_tokens > 0 && (!s->pos_dev || !s->slot_dev)))
+        return fail(PC_ERR_INVALID_ARG, "bad pc_kv_tables arguments");
+    if (s->page_size < 8 || s->page_size % 8 || s->page_size > (1 << 16))
+        return fail(PC_ERR_FORMAT, "page_size must be a multiple of 8, at most 65536");
+    if (s->n_requests > (1 << 20) || s->n_tokens > (1 << 28) || (int64_t)s->max_pages * s->page_size > INT_MAX / 2)
+        return fail(PC_ERR_RANGE, "too many requests, tokens or positions");
+    if (s->kv_end_dev == s->kv_len_dev || s->n_free_out_dev == s->n_free_dev)
+        return fail(PC_ERR_INVALID_ARG, "kv_end and n_free_out must not overlap the inputs");
+    OnDevice on(device);
+    PC_CU(on.e);
+    PC_CU(launch_kv_tables(*s, (cudaStream_t)stream));
+    return PC_OK;
+}
+
+pc_status pc_kv_store(int device, const pc_kv_pages *kv, const void *k_dev, const int64_t *k_stride,
+                      const void *v_dev, const int64_t *v_stride, int src_dtype, const int64_t *slot_dev, int n,
+                      void *stream) {
+    PC_TRY(check_pages(kv));
+    if (n < 0) return fail(PC_ERR_INVALID_ARG, "bad pc_kv_store arguments");
+    if (!dt_ok(src_dtype)) return fail(PC_ERR_FORMAT, "source type must be PC_DT_F32, PC_DT_F16 or PC_DT_BF16");
+    if (n == 0) return PC_OK;
+    if (!k_dev || !v_dev || !k_stride || !v_stride || !slot_dev)
+        return fail(PC_ERR_INVALID_ARG, "bad pc_kv_store arguments");
+    if (!aligned(k_dev, k_stride, 2, dt_size(src_dtype)) || !aligned(v_dev, v_stride, 2, dt_size(src_dtype)))
+        return fail(PC_ERR_FORMAT, "k and v need 16-byte aligned pointers and strides");
+    OnDevice on(device);
+    PC_CU(on.e);
+    int nsm = 148;
+    PC_CU(cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, device));
+    PC_CU(launch_kv_store(*kv, k_dev, k_stride, v_dev, v_stride, src_dtype, slot_dev, n, nsm, (cudaStream_t)stream));
+    return PC_OK;
+}
+
+pc_status pc_attn_create(int device, pc_attn **out) {
+    if (!out) return fail(PC_ERR_INVALID_ARG, "bad pc_attn_create arguments");
+    OnDevice on(device);
+    PC_CU(on.e);
+    pc_attn *a = new pc_attn();
+    a->dev = device;
+    auto done = [&](pc_status s) {
+        if (s != PC_OK) pc_attn_free(a);
+        else *out = a;
+        return s;
+    };
+    cudaError_t e = cudaDeviceGetAttribute(&a->nsm, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&a->max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+    if (e == cudaSuccess) e = attn_simt_configure();
+    if (e == cudaSuccess) e = cudaMalloc(&a->part, attn_part_floats(a->nsm) * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&a->ticket, ATTN_MAX_CTAS * sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMalloc(&a->err, sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(a->ticket, 0, ATTN_MAX_CTAS * sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMemset(a->err, 0, sizeof(int));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    return done(e == cudaSuccess ? PC_OK : cuda_fail(e, "pc_attn_create"));
+}
+
+void pc_attn_free(pc_attn *a) {
+    if (!a) return;
+    OnDevice on(a->dev);
+    cudaDeviceSynchronize();
+    cudaFree(a->part);
+    cudaFree(a->ticket);
+    cudaFree(a->err);
+    delete a;
+}
+
+pc_status pc_attn_paged(pc_attn *a, const pc_attn_call *c, const pc_kv_pages *kv, const int *page_table_dev,
+                        int max_pages, const int *kv_len_dev, void *stream) {
+    if (!a) return fail(PC_ERR_INVALID_ARG, "null pc_attn");
+    PC_TRY(check_call(c));
+    PC_TRY(check_pages(kv));
+    if (c->n_rows == 0 || c->n_requests == 0) return PC_OK;
+    if (!page_table_dev || !kv_len_dev || max_pages < 1)
+        return fail(PC_ERR_INVALID_ARG, "bad pc_attn_paged arguments");
+    if (kv->dtype != c->dtype || kv->n_kv_heads != c->n_kv_heads || kv->head_dim != c->head_dim)
+        return fail(PC_ERR_FORMAT, "q and the cache differ in type, KV heads or head_dim");
+    if ((int64_t)max_pages * kv->page_size > INT_MAX / 2) return fail(PC_ERR_RANGE, "too many positions");
+    OnDevice on(a->dev);
+    PC_CU(on.e);
+    AttnOp o = op_of(a, c);
+    o.k = kv->k_dev;
+    o.v = kv->v_dev;
+    for (int i = 0; i < 3; ++i) {
+        o.ks[i] = kv->k_stride[i];
+        o.vs[i] = kv->v_stride[i];
+    }
+    o.table = page_table_dev;
+    o.kv_len = kv_len_dev;
+    o.max_pages = max_pages;
+    o.page_size = kv->page_size;
+    o.n_pages = kv->n_pages;
+    return run_attention(a, o, c->dtype, (cudaStream_t)stream);
+}
+
+pc_status pc_attn_packed(pc_attn *a, const pc_attn_call *c, const void *k_dev, const int64_t *k_stride,
+                         const void *v_dev, const int64_t *v_stride, void *stream) {
+    if (!a) return fail(PC_ERR_INVALID_ARG, "null pc_attn");
+    PC_TRY(check_call(c));
+    if (c->n_rows == 0 || c->n_requests == 0) return PC_OK;
+    if (!k_dev || !v_dev || !k_stride || !v_stride) return fail(PC_ERR_INVALID_ARG, "null tensor");
+    const int es = dt_size(c->dtype);
+    if (!aligned(k_dev, k_stride, 2, es) || !aligned(v_dev, v_stride, 2, es))
+        return fail(PC_ERR_FORMAT, "k and v need 16-byte aligned pointers and strides");
+    OnDevice on(a->dev);
+    PC_CU(on.e);
+    AttnOp o = op_of(a, c);
+    o.k = k_dev;
+    o.v = v_dev;
+    for (int i = 0; i < 2; ++i) {
+        o.ks[i + 1] = k_stride[i];
+        o.vs[i + 1] = v_stride[i];
+    }
+    return run_attention(a, o, c->dtype, (cudaStream_t)stream);
+}
+
+pc_status pc_attn_check(pc_attn *a, void *stream) {
+    if (!a) return fail(PC_ERR_INVALID_ARG, "null pc_attn");
+    OnDevice on(a->dev);
+    PC_CU(on.e);
+    PC_CU(cudaStreamSynchronize((cudaStream_t)stream));
+    int e = 0;
+    PC_CU(cudaMemcpy(&e, a->err, sizeof e, cudaMemcpyDeviceToHost));
+    if (!e) return PC_OK;
+    PC_CU(cudaMemset(a->err, 0, sizeof e));
+    PC_CU(cudaDeviceSynchronize());
+    return fail(PC_ERR_TIMEOUT, "a bounded wait of an attention kernel gave up");
+}
+
+}  // extern "C"
