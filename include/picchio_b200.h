@@ -389,7 +389,7 @@ typedef struct {
     const int *cu_new_dev; /* [n_requests + 1], from 0, ascending */
     const float *sinks_dev; /* [n_heads] or NULL */
     int window;            /* positions a row sees, itself included; 0: all */
-    float scale;           /* 1 / sqrt(head_dim) as a rule */
+    float scale;           /* above 0; 1 / sqrt(head_dim) as a rule */
 } pc_attn_call;
 
 /* Workspace of the attention calls on one GPU: what the thread blocks that

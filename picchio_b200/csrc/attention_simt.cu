@@ -250,17 +250,18 @@ __global__ void __launch_bounds__(SimtCfg<HDP, R>::THREADS) attn_simt_kernel(con
             const int f = g.r0 + 4 * ty + i;
             if (f >= g.r1) continue;
             const int h = w.kvh * a.G + f % a.G;
+            const bool none = m[i] == -INFINITY && l[i] == 0.0f;  // no key seen
             float corr = 1.0f, total = l[i];
             if (a.sinks) {
                 const float sk = a.sinks[h], mm = fmaxf(m[i], sk);
                 corr = m[i] == -INFINITY ? 0.0f : expf(__fsub_rn(m[i], mm));
                 total = __fmaf_rn(l[i], corr, expf(__fsub_rn(sk, mm)));
             }
-            const float inv = m[i] == -INFINITY ? 0.0f : __fdiv_rn(corr, total);
+            const float inv = none ? 0.0f : __fdiv_rn(corr, total);
             T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.s.q0 + f / a.G) * a.os[0] + (int64_t)h * a.os[1];
 #pragma unroll
             for (int d = 0; d < DPT; ++d)
-                if (tx + TX * d < a.D) from_f(out[tx + TX * d], m[i] == -INFINITY ? 0.0f : __fmul_rn(o[i][d], inv));
+                if (tx + TX * d < a.D) from_f(out[tx + TX * d], none ? 0.0f : __fmul_rn(o[i][d], inv));
         }
     }
 }
@@ -296,7 +297,7 @@ cudaError_t simt_set_all() {
 
 }  // namespace
 
-size_t attn_part_floats(int nsm) {
+size_t attn_simt_part_floats(int nsm) {
     return (size_t)nsm * 2 * 3 * SimtCfg<128, 64>::PART;
 }
 

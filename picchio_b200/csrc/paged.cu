@@ -2,7 +2,9 @@
 // their arguments, the attention workspace, and the choice of a kernel.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -60,7 +62,8 @@ pc_status check_pages(const pc_kv_pages *kv) {
 }
 
 pc_status check_call(const pc_attn_call *c) {
-    if (!c || c->n_rows < 0 || c->n_requests < 0 || c->n_heads < 1 || c->n_kv_heads < 1 || c->window < 0)
+    if (!c || c->n_rows < 0 || c->n_requests < 0 || c->n_heads < 1 || c->n_kv_heads < 1 || c->window < 0 ||
+        !(c->scale > 0.0f) || !std::isfinite(c->scale))
         return fail(PC_ERR_INVALID_ARG, "bad pc_attn_call");
     if (c->n_heads % c->n_kv_heads) return fail(PC_ERR_INVALID_ARG, "n_heads must be a multiple of n_kv_heads");
     if (c->n_heads / c->n_kv_heads > 128) return fail(PC_ERR_FORMAT, "at most 128 query heads per KV head");
@@ -105,7 +108,9 @@ AttnOp op_of(const pc_attn *a, const pc_attn_call *c) {
 }
 
 pc_status run_attention(pc_attn *a, const AttnOp &o, int dtype, cudaStream_t st) {
-    PC_CU(launch_attn_simt(o, dtype, a->nsm, st));
+    cudaError_t e = cudaSuccess;
+    if (dtype == PC_DT_F32 || !launch_attn_rows(o, dtype, a->nsm, st, e)) e = launch_attn_simt(o, dtype, a->nsm, st);
+    PC_CU(e);
     return PC_OK;
 }
 
@@ -164,7 +169,9 @@ pc_status pc_attn_create(int device, pc_attn **out) {
     cudaError_t e = cudaDeviceGetAttribute(&a->nsm, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&a->max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
     if (e == cudaSuccess) e = attn_simt_configure();
-    if (e == cudaSuccess) e = cudaMalloc(&a->part, attn_part_floats(a->nsm) * sizeof(float));
+    if (e == cudaSuccess) e = attn_rows_configure();
+    const size_t part = std::max(attn_simt_part_floats(a->nsm), attn_rows_part_floats(a->nsm));
+    if (e == cudaSuccess) e = cudaMalloc(&a->part, part * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&a->ticket, ATTN_MAX_CTAS * sizeof(unsigned));
     if (e == cudaSuccess) e = cudaMalloc(&a->err, sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(a->ticket, 0, ATTN_MAX_CTAS * sizeof(unsigned));

@@ -29,10 +29,16 @@ struct AttnOp {
 
 constexpr int ATTN_MAX_CTAS = 148 * 8;
 
-// Workspace floats that any of the kernels needs for `nsm` SMs.
-size_t attn_part_floats(int nsm);
+// Workspace floats that the kernel needs for `nsm` SMs.
+size_t attn_simt_part_floats(int nsm);
 cudaError_t attn_simt_configure();
 cudaError_t launch_attn_simt(const AttnOp &a, int dtype, int nsm, cudaStream_t st);
+
+// f16 and bf16 on the tensor cores; false (nothing launched) if K or V has
+// strides that no tensor map describes.
+size_t attn_rows_part_floats(int nsm);
+cudaError_t attn_rows_configure();
+bool launch_attn_rows(const AttnOp &a, int dtype, int nsm, cudaStream_t st, cudaError_t &e);
 
 cudaError_t launch_kv_tables(const pc_kv_step &s, cudaStream_t st);
 cudaError_t launch_kv_store(const pc_kv_pages &kv, const void *k, const int64_t *ks, const void *v, const int64_t *vs,

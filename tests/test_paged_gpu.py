@@ -280,9 +280,11 @@ def test_unseen_keys_have_no_part(dtype, D):
         out = handle().packed(q, k, v, cu, window=window)
         want, bound = reference(q, k, v, 0, None, window, D ** -0.5, dtype)
         close(out, want, bound)
+    q[5, 1] = float("nan")
     k[250] = float("nan")
     clean = handle().packed(q, k, v, cu)
-    assert torch.isfinite(clean[:37].float()).all()
+    assert torch.isnan(clean[5, 1].float()).all()
+    assert torch.isfinite(clean[:5].float()).all() and torch.isfinite(clean[6:37].float()).all()
     assert torch.isfinite(clean[:200, 2].float()).all() and torch.isnan(clean[250:].float()).all()
 
 
