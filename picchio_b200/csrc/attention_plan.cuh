@@ -23,6 +23,12 @@
 
 namespace pc {
 
+// f / G for the flat row f = token * G + head of a group of G heads (f * G <
+// 2^32, checked on the host)
+__device__ __forceinline__ int div_g(const AttnOp &a, int f) {
+    return a.G == 1 ? f : (int)__umulhi((unsigned)f, a.inv_g);
+}
+
 // A request's rows and keys as every kernel reads them, safe for any input.
 struct SeqGeo {
     int q0, qlen, kv, p0, n_items;  // first row, rows, keys, first row's position (may be < 0), items
@@ -53,8 +59,8 @@ __device__ __forceinline__ ItemGeo item_geo(const AttnOp &a, const SeqGeo &s, in
     ItemGeo g;
     g.r0 = item * R;
     g.r1 = min(g.r0 + R, s.qlen * a.G);
-    g.pmin = s.p0 + g.r0 / a.G;
-    g.pmax = s.p0 + (g.r1 - 1) / a.G;
+    g.pmin = s.p0 + div_g(a, g.r0);
+    g.pmax = s.p0 + div_g(a, g.r1 - 1);
     g.kb = a.window > 0 ? max(0, g.pmin - a.window + 1) : 0;
     g.ke = max(g.pmax + 1, 0);
     g.t0 = g.kb / KT;
@@ -212,9 +218,9 @@ struct PlanWalk {
         first = true;
     }
     // false: the share is done.  Sets tl, th, s, g for the item at hand.
-    __device__ __forceinline__ bool load() {
+    __device__ __forceinline__ bool load(bool request = true) {
         if (b >= a.B) return false;
-        s = seq_geo<R>(a, b);
+        if (request) s = seq_geo<R>(a, b);
         while (s.n_items == 0) {
             if (++b >= a.B) return false;
             s = seq_geo<R>(a, b);
@@ -229,14 +235,16 @@ struct PlanWalk {
     __device__ __forceinline__ bool next() {
         if (b == sh.e.b && kvh == sh.e.kvh && item == sh.e.item) return false;  // cut here
         first = false;
+        bool request = false;
         if (++item == s.n_items) {
             item = 0;
             if (++kvh == a.KVH) {
                 kvh = 0;
                 ++b;
+                request = true;
             }
         }
-        return load();
+        return load(request);
     }
     __device__ __forceinline__ bool whole() const { return tl == 0 && th == g.nt; }
 };

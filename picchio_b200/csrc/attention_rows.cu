@@ -8,15 +8,30 @@
 //                   running maximum and sum, weights back to TMEM, and at the
 //                   end of an item the output
 //   warp 8          K and V tiles by TMA into a ring (one box per page piece)
-//   warp 9          tcgen05.mma: S = Q K^T (both from shared memory), O += P V
-//                   (P from TMEM, V from shared memory as it lies: keys are
-//                   the strided, head columns the contiguous dimension)
-//   warps 10, 11    Q rows of the next item; V rows of masked tiles put in
+//   warp 9          tcgen05.mma: S = Q K^T, both from shared memory
+//   warp 11         tcgen05.mma: O += P V, P from TMEM, V from shared memory as
+//                   it lies (keys are the strided, head columns the
+//                   contiguous dimension)
+//   warp 10         Q rows of the next item; V rows of masked tiles put in
 //                   order (below)
-// With two row tiles one is in the softmax while the other's products run.
-// At head sizes to 64, S, P and O of both tiles fit TMEM's 512 columns side
-// by side, so the next S is computed while a row group is still in its
-// exponentials; at 128, P takes the place of its S.
+// P takes the place of its S in TMEM.  Beside O (2 x head size columns) there
+// is room for three such buffers at head sizes to 64 and for two at 128; they
+// go round the row tiles in turn, so while one row tile is in the softmax, the
+// other's products run, and with three the next S is ready before its row
+// tile has finished.
+// The softmax reads S twice (maximum, then weights, 32 columns at a time)
+// instead of keeping it in registers: the unrolled form of 900 instructions a
+// tile did not fit the instruction cache and spent more time waiting for
+// instructions than issuing them.
+//
+// The exponentials are the softmax's cost: at head size 64 a tile pair's
+// products take 1024 tensor cycles and its 32,768 exponentials 2048 cycles of
+// the special-function units (16 a cycle).  So in tiles without masked keys a
+// part of them runs on the FMA units instead: 2^x = 2^n 2^f, n the nearest
+// integer, 2^f on [-1/2, 1/2] by a polynomial of degree 3 (bf16 weights; its
+// relative error 7.5e-5 is 1/26 of the weight's rounding to bf16) or 4 (f16;
+// 2.7e-6, 1/90), fitted by reweighted least squares to the least maximal
+// relative error.
 //
 // The maximum that weights are taken against is moved only when a row's
 // maximum has grown by more than 2^8 (any reference within the exponent
@@ -29,6 +44,8 @@
 // from global memory at the end of the item.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "attention_plan.cuh"
 #include "launch.cuh"
@@ -47,15 +64,20 @@ struct RowsCfg {
     static constexpr int PANELS = HD / 64;        // 64-column (128-byte) panels of a row
     static constexpr int TILE = PANELS * 16384;   // bytes of 128 rows
     static constexpr int STAGES = HD == 64 ? 3 : 2;
-    static constexpr bool ALIAS = HD == 128;      // P in the place of S
-    static constexpr int S0 = 0, P0 = ALIAS ? 0 : 256, PSTEP = ALIAS ? 128 : 64, O0 = ALIAS ? 256 : 384;
-    static constexpr size_t SMEM = 1024 + (size_t)TILE * (2 + 2 * STAGES);
+    static constexpr int QB = HD == 64 ? 2 : 1;   // Q buffers
+    static constexpr int NB = HD == 64 ? 3 : 2;   // S / P buffers in TMEM, 128 columns each
+    static constexpr int O0 = NB * 128;
+    static constexpr size_t SMEM = 1024 + (size_t)TILE * (2 * QB + 2 * STAGES) + 8 * 2048;  // 2 KB a row warp: output
     static constexpr int PART = RW_R * (HD + 2);
 };
 
+struct KeySteps {
+    int lo, hi;
+};
+
 struct RowsBars {
-    uint64_t q_full[2], q_free[2], s_full[2], s_free[2], p_full[2], o_full[2];
-    uint64_t k_full[3], k_free[3], v_full[3], v_free[3], v_fixed[3], both, drain;
+    uint64_t q_full[4], q_free[4], s_full[3], p_full[3], o_full[4];
+    uint64_t k_full[3], k_free[3], v_full[3], v_free[3], v_fixed[3], both, drain[2];
 };
 
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
@@ -87,6 +109,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
           "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
+}
+// Waits for this thread's TMEM loads; the values pass through it, so that no
+// use of them is scheduled before.
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), 
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                   "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
     asm volatile(
@@ -123,6 +163,99 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// mbar_try_wait that may sleep up to 20 us: a waiting warp issues nothing
+// that the row warps of its scheduler would have to wait for
+__device__ __forceinline__ bool mbar_sleep_wait(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// Whether a phase is complete, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// One lane of the warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// The same value in all lanes, known as such to the compiler
+template <typename V>
+__device__ __forceinline__ V uniform(V v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Bits y of 32 with lo < y <= hi
+__device__ __forceinline__ uint32_t seen_bits(int lo, int hi) {
+    const uint32_t up = hi >= 31 ? ~0u : hi < 0 ? 0u : (2u << hi) - 1u;
+    const uint32_t dn = lo >= 31 ? ~0u : lo < 0 ? 0u : (2u << lo) - 1u;
+    return up & ~dn;
+}
+
+// -inf in the place of scores that are not seen
+__device__ __forceinline__ void hide(uint32_t (&sv)[32], uint32_t seen) {
+#pragma unroll
+    for (int y = 0; y < 32; ++y)
+        if (!(seen >> y & 1u)) sv[y] = 0xFF800000u;
+}
+
+__device__ __forceinline__ uint64_t f2_pack_bits(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) { return f2_pack_bits(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float f2_lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float f2_hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_ex2(uint64_t v) { return f2_pack(ex2(f2_lo(v)), ex2(f2_hi(v))); }
+// the largest of three, NaN if one of them is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+constexpr int RW_POLY = 6;  // of 16 pairs of exponentials, those on the FMA units
+
+// 2^x of both lanes: n = round(x) by adding 1.5 * 2^23, 2^(x - n) by a
+// polynomial (coefficients c[0] ...), n into the exponent.  x from -125 on (a
+// weight below 2^-125 of the largest counts as that) to 127.
+template <int DEG>
+__device__ __forceinline__ uint64_t f2_pow2(uint64_t x, const float (&c)[DEG + 1]) {
+    const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
+    x = f2_pack(fmaxf(f2_lo(x), -125.0f), fmaxf(f2_hi(x), -125.0f));
+    const uint64_t t = f2_add(x, magic), f = f2_sub(x, f2_sub(t, magic));
+    uint64_t p = f2_pack(c[DEG], c[DEG]);
+#pragma unroll
+    for (int i = DEG - 1; i >= 0; --i) p = f2_fma(p, f, f2_pack(c[i], c[i]));
+    return f2_pack_bits((uint32_t)p + ((uint32_t)t << 23), (uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23));
+}
+
 // Element types: instruction-descriptor code, packing, the bits of a
 // non-finite exponent, and the power of two that weights are stored at (f16
 // weights keep 7 binary orders more before they underflow; the sums carry
@@ -139,6 +272,9 @@ struct Half16<__nv_bfloat16> {
         return r;
     }
     static __device__ __forceinline__ float up(uint32_t h) { return __uint_as_float(h << 16); }
+    static __device__ __forceinline__ uint64_t pow2(uint64_t x) {
+        return f2_pow2<3>(x, {0.9999280571937561f, 0.6932609677314758f, 0.2426111251115799f, 0.0551716685295105f});
+    }
 };
 template <>
 struct Half16<__half> {
@@ -150,18 +286,22 @@ struct Half16<__half> {
         return r;
     }
     static __device__ __forceinline__ float up(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)h)); }
+    static __device__ __forceinline__ uint64_t pow2(uint64_t x) {
+        return f2_pow2<4>(x, {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f, 0.05591785907745361f,
+                              0.009570102207362652f});
+    }
 };
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(RW_THREADS, 1)
     attn_rows_kernel(const AttnOp a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                     const int box) {
+                     const __grid_constant__ CUtensorMap qmap, const int box, const bool qtma) {
     using C = RowsCfg<HD>;
     using E = Half16<T>;
-    constexpr int NS = C::STAGES;
+    constexpr int NS = C::STAGES, QB = C::QB;
     extern __shared__ uint8_t rows_smem_raw[];
     uint8_t *smem = rows_smem_raw + (1024 - (smem_u32(rows_smem_raw) & 1023)) % 1024;
-    uint8_t *qs = smem, *ks = qs + 2 * C::TILE, *vs = ks + NS * C::TILE;
+    uint8_t *qs = smem, *ks = qs + 2 * C::QB * C::TILE, *vs = ks + NS * C::TILE, *os = vs + NS * C::TILE;
     __shared__ PlanScratch<RW_THREADS> sc;
     __shared__ RowsBars bar;
     __shared__ uint32_t tmem_slot;
@@ -171,23 +311,25 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int t = 0; t < 2; ++t) {
-            mbar_init(&bar.q_full[t], 64);
+        for (int t = 0; t < 4; ++t) {
+            mbar_init(&bar.q_full[t], 1);
             mbar_init(&bar.q_free[t], 1);
-            mbar_init(&bar.s_full[t], 1);
-            mbar_init(&bar.s_free[t], 128);
-            mbar_init(&bar.p_full[t], 128);
-            mbar_init(&bar.o_full[t], 1);
         }
+        for (int b = 0; b < C::NB; ++b) {
+            mbar_init(&bar.s_full[b], 1);
+            mbar_init(&bar.p_full[b], 128);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&bar.o_full[i], 1);
         for (int s = 0; s < NS; ++s) {
             mbar_init(&bar.k_full[s], 1);
             mbar_init(&bar.k_free[s], 1);
             mbar_init(&bar.v_full[s], 1);
             mbar_init(&bar.v_free[s], 1);
-            mbar_init(&bar.v_fixed[s], 64);
+            mbar_init(&bar.v_fixed[s], 32);
         }
         mbar_init(&bar.both, 256);
-        mbar_init(&bar.drain, 1);
+        mbar_init(&bar.drain[0], 1);
+        mbar_init(&bar.drain[1], 1);
         fence_mbar_init();
         dead = 0;
         for (int i = 0; i < 4; ++i) odd[i] = 0;
@@ -206,9 +348,9 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
 
     // A bounded wait: false once it, or any other wait of the block, gave up.
     auto wait = [&](uint64_t *b, uint32_t parity) -> bool {
-        if (mbar_try_wait(b, parity)) return true;
+        if (mbar_sleep_wait(b, parity)) return true;
         const long long t0 = clock64();
-        while (!mbar_try_wait(b, parity)) {
+        while (!mbar_sleep_wait(b, parity)) {
             if (dead) return false;
             if (clock64() - t0 > RW_WAIT_CLOCKS) {
                 dead = 1;
@@ -217,6 +359,25 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             }
         }
         return true;
+    };
+    auto wait_all = [&](uint64_t *b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    // the steps of 16 keys of a tile that hold keys of the item (one at least)
+    auto key_steps = [&](const ItemGeo &g, int t) -> KeySteps {
+        const int k0 = (g.t0 + t) * RW_KT;
+        KeySteps k;
+        k.lo = max(g.kb - k0, 0) / 16;
+        k.hi = min(max((g.ke - k0 + 15) / 16, k.lo + 1), RW_KT / 16);
+        return k;
+    };
+    // after a failure: products in flight end before TMEM is freed
+    auto drain = [&](bool ok, uint64_t *b) {
+        if (!ok && elect_one()) {
+            tc_commit(b);
+            const long long t0 = clock64();
+            while (!mbar_try_wait(b, 0))
+                if (clock64() - t0 > RW_WAIT_CLOCKS) break;
+        }
+        __syncwarp();
     };
     // a tile of keys that some row of the item does not see whole
     auto masked = [&](const ItemGeo &g, int t) -> bool {
@@ -229,10 +390,25 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
     } else if (warp == 8) {
         // ---- K and V tiles ----
         PlanWalk<RW_R, RW_KT> w(a, sc.share);
-        int it = 0, fills[2] = {0, 0};
+        int it = 0, item = 0, fills[2] = {0, 0};
         bool ok = true;
-        for (bool more = w.load(); more && ok; more = w.next()) {
+        auto load_q = [&]() {
+            for (int t = 0; t < 2; ++t) {
+                const int b = item % QB * 2 + t;
+                if (item >= QB && !(ok = wait_all(&bar.q_free[b], (item / QB - 1) & 1))) return;
+                if (lane == 0) mbar_arrive_expect_tx(&bar.q_full[b], C::TILE);
+                __syncwarp();
+                if (lane < C::PANELS)
+                    tma_load_3d(qs + b * C::TILE + lane * 16384, &qmap, &bar.q_full[b], lane * 64, w.kvh * a.G,
+                                w.s.q0 + div_g(a, w.g.r0 + t * 128));
+                __syncwarp();
+            }
+        };
+        for (bool more = w.load(); more && ok; more = w.next(), ++item) {
+            if (qtma && QB > 1) load_q();
             for (int t = w.tl; t < w.th && ok; ++t, ++it) {
+                // one Q buffer: the item's first K and V need not wait for it
+                if (qtma && QB == 1 && t == w.tl + 1) load_q();
                 const int s = it % NS;
                 const uint32_t ph = (it / NS) & 1;
                 const int k0 = (w.g.t0 + t) * RW_KT;
@@ -241,8 +417,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 const int nb = max(hi - lo, 0);
                 for (int kv = 0; kv < 2 && ok; ++kv) {
                     uint64_t *full = kv ? &bar.v_full[s] : &bar.k_full[s];
-                    ok = wait(kv ? &bar.v_free[s] : &bar.k_free[s], ph ^ 1);
-                    ok = __all_sync(0xffffffffu, ok);
+                    ok = wait_all(kv ? &bar.v_free[s] : &bar.k_free[s], ph ^ 1);
                     if (!ok) break;
                     uint8_t *dst = (kv ? vs : ks) + s * C::TILE;
                     const CUtensorMap *map = kv ? &vmap : &kmap;
@@ -256,7 +431,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                         const int p = i / nb, row = (lo + i % nb) * box, key = k0 + row;
                         uint8_t *d = dst + p * 16384 + row * 128;
                         if (a.table) {
-                            const int page = __ldg(a.table + (int64_t)w.b * a.max_pages + key / a.page_size);
+                            const int page = a.table[(int64_t)w.b * a.max_pages + key / a.page_size];
                             tma_load_4d(d, map, full, p * 64, key % a.page_size, w.kvh, page);
                         } else {
                             tma_load_3d(d, map, full, p * 64, w.s.q0 + key, w.kvh);
@@ -265,6 +440,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                     __syncwarp();
                 }
             }
+            if (qtma && QB == 1 && w.th == w.tl + 1 && ok) load_q();
         }
         if (!ok && lane == 0)  // copies in flight land before the block ends
             for (int s = 0; s < NS; ++s)
@@ -276,125 +452,175 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                             if (clock64() - t0 > RW_WAIT_CLOCKS) break;
                 }
     } else if (warp == 9) {
-        // ---- products ----
-        if (lane == 0) {
-            constexpr uint32_t ID_QK = (1u << 4) | (E::FMT << 7) | (E::FMT << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-            constexpr uint32_t ID_PV = (1u << 4) | (E::FMT << 7) | (E::FMT << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) |
-                                       ((128u >> 4) << 24);
-            PlanWalk<RW_R, RW_KT> w(a, sc.share);
-            int kit = 0, vit = 0, n = 0, item = 0;  // n: tiles begun (S of both row tiles)
-            bool ok = true;
-            auto qk = [&](int t, int s) {  // S[t] = Q[t] K^T
-                const uint64_t qd = sw128_desc(qs + t * C::TILE), kd = sw128_desc(ks + s * C::TILE);
+        // ---- S = Q K^T ----
+        // The whole warp walks, one elected lane issues: what the instructions
+        // take stays in uniform registers.  A product's issue holds the warp
+        // for as long as the tensor core takes it, so the other products have
+        // their own warp, and each prepares its next while the other's run.
+        constexpr uint32_t ID = (1u << 4) | (E::FMT << 7) | (E::FMT << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+        const uint32_t tmu = uniform(tm);
+        const uint64_t qd0 = sw128_desc(qs), kd0 = sw128_desc(ks);
+        PlanWalk<RW_R, RW_KT> w(a, sc.share);
+        int n = 0, sbuf = 0, qbuf = 0, kst = 0;
+        uint32_t qph = 0, kph = 0;
+        bool ok = true;
+        for (bool more = w.load(); more && ok; more = w.next()) {
+            const int left = uniform(w.th - w.tl);
+            for (int j = 0; j < left && ok; ++j) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const int off = (k / 4) * (16384 >> 4) + (k % 4) * 2;
-                    tc_mma_f16(tm + C::S0 + t * 128, qd + off, kd + off, ID_QK, k > 0);
+                for (int t = 0; t < 2; ++t, ++n) {
+                    if (j == 0 && !(ok = wait_all(&bar.q_full[qbuf * 2 + t], qph))) break;
+                    if (t == 0 && !(ok = wait_all(&bar.k_full[kst], kph))) break;
+                    // the buffer's last P has met its V
+                    if (n >= C::NB && !(ok = wait_all(&bar.o_full[(n - C::NB) & 3], (n - C::NB) >> 2 & 1))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t qd = qd0 + (qbuf * 2 + t) * (C::TILE >> 4), kd = kd0 + kst * (C::TILE >> 4);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const int off = (k / 4) * (16384 >> 4) + (k % 4) * 2;
+                            tc_mma_f16(tmu + sbuf * 128, qd + off, kd + off, ID, k > 0);
+                        }
+                        tc_commit(&bar.s_full[sbuf]);
+                        if (j + 1 == left) tc_commit(&bar.q_free[qbuf * 2 + t]);
+                        if (t == 1) tc_commit(&bar.k_free[kst]);
+                    }
+                    __syncwarp();
+                    if (++sbuf == C::NB) sbuf = 0;
                 }
-                tc_commit(&bar.s_full[t]);
-            };
-            auto pv = [&](int t, int s, bool acc) {  // O[t] (+)= P[t] V
-#pragma unroll
-                for (int k = 0; k < RW_KT / 16; ++k)
-                    tc_mma_ts(tm + C::O0 + t * HD, tm + C::P0 + t * C::PSTEP + k * 8,
-                              sw128_desc_n(smem_u32(vs + s * C::TILE) + k * 2048, 16384), ID_PV, acc || k > 0);
-                tc_commit(&bar.o_full[t]);
-            };
-            for (bool more = w.load(); more && ok; more = w.next(), ++item) {
-                for (int j = w.tl - 1; j < w.th && ok; ++j) {
-                    // S of tile j + 1
-                    auto next_s = [&](int t) -> bool {
-                        if (j + 1 >= w.th) return true;
-                        if (j + 1 == w.tl && !wait(&bar.q_full[t], item & 1)) return false;
-                        if (t == 0 && !wait(&bar.k_full[kit % NS], (kit / NS) & 1)) return false;
-                        if (!C::ALIAS && n > 0 && !wait(&bar.s_free[t], (n - 1) & 1)) return false;
-                        tc_fence_after();
-                        qk(t, kit % NS);
-                        if (j + 2 == w.th) tc_commit(&bar.q_free[t]);
-                        if (t == 1) {
-                            tc_commit(&bar.k_free[kit % NS]);
-                            ++kit;
-                            ++n;
-                        }
-                        return true;
-                    };
-                    auto this_o = [&](int t) -> bool {
-                        if (j < w.tl) return true;
-                        const int s = vit % NS;
-                        if (t == 0 && !wait(&bar.v_full[s], (vit / NS) & 1)) return false;
-                        if (t == 0 && !wait(&bar.v_fixed[s], (vit / NS) & 1)) return false;
-                        if (!wait(&bar.p_full[t], vit & 1)) return false;
-                        tc_fence_after();
-                        pv(t, s, j > w.tl);
-                        if (t == 1) {
-                            tc_commit(&bar.v_free[s]);
-                            ++vit;
-                        }
-                        return true;
-                    };
-                    if (C::ALIAS) ok = this_o(0) && next_s(0) && this_o(1) && next_s(1);
-                    else ok = next_s(0) && next_s(1) && this_o(0) && this_o(1);
+                if (++kst == NS) {
+                    kst = 0;
+                    kph ^= 1;
                 }
             }
-            if (!ok) {  // products in flight end before TMEM is freed
-                tc_commit(&bar.drain);
-                const long long t0 = clock64();
-                while (!mbar_try_wait(&bar.drain, 0))
-                    if (clock64() - t0 > RW_WAIT_CLOCKS) break;
+            if (++qbuf == QB) {
+                qbuf = 0;
+                qph ^= 1;
             }
         }
-        __syncwarp();
-    } else if (warp >= 10) {
-        // ---- Q rows, V rows of masked tiles ----
-        const int ht = tid - 320;
+        drain(ok, &bar.drain[0]);
+    } else if (warp == 11) {
+        // ---- O += P V ----
+        constexpr uint32_t ID = (1u << 4) | (E::FMT << 7) | (E::FMT << 10) | (1u << 16) | (((uint32_t)HD >> 3) << 17) |
+                                ((128u >> 4) << 24);
+        const uint32_t tmu = uniform(tm);
+        const uint64_t vd0 = sw128_desc_n(smem_u32(vs), 16384);
         PlanWalk<RW_R, RW_KT> w(a, sc.share);
-        int it = 0, item = 0;
+        int n = 0, pbuf = 0, vst = 0;
+        uint32_t pph = 0, vph = 0;
         bool ok = true;
-        for (bool more = w.load(); more && ok; more = w.next(), ++item) {
-            const T *q = reinterpret_cast<const T *>(a.q) + (int64_t)w.s.q0 * a.qs[0] + (int64_t)w.kvh * a.G * a.qs[1];
-            for (int t = 0; t < 2 && ok; ++t) {
-                ok = item == 0 || wait(&bar.q_free[t], (item - 1) & 1);
-                if (!ok) break;
-                const uint32_t dst = smem_u32(qs + t * C::TILE);
-                for (int i = ht; i < 128 * C::PANELS * 8; i += 64) {
-                    const int r = i / (C::PANELS * 8), c = i % (C::PANELS * 8), f = w.g.r0 + t * 128 + r;
-                    const bool in = f < w.g.r1 && c * 8 < a.D;
-                    const int fc = in ? f : 0, cc = in ? c : 0;
-                    cp_async16_fill(dst + (c / 8) * 16384 + r * 128 + (((c % 8) ^ (r & 7)) << 4),
-                                    q + (int64_t)(fc / a.G) * a.qs[0] + (int64_t)(fc % a.G) * a.qs[1] + cc * 8,
-                                    in ? 16 : 0);
+        for (bool more = w.load(); more && ok; more = w.next()) {
+            const int left = uniform(w.th - w.tl);
+            for (int j = 0; j < left && ok; ++j) {
+                const KeySteps ks_ = key_steps(w.g, w.tl + j);
+                const int k0 = uniform(ks_.lo), k1 = uniform(ks_.hi);
+                // V in order implies V there
+                if (!(ok = wait_all(&bar.v_fixed[vst], vph))) break;
+#pragma unroll
+                for (int t = 0; t < 2; ++t, ++n) {
+                    if (!(ok = wait_all(&bar.p_full[pbuf], pph))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t vd = vd0 + vst * (C::TILE >> 4);
+#pragma unroll
+                        for (int k = 0; k < RW_KT / 16; ++k)
+                            if (k >= k0 && k < k1)
+                                tc_mma_ts(tmu + C::O0 + t * HD, tmu + pbuf * 128 + k * 8, vd + k * (2048 >> 4), ID,
+                                          j > 0 || k > k0);
+                        tc_commit(&bar.o_full[n & 3]);
+                        if (t == 1) tc_commit(&bar.v_free[vst]);
+                    }
+                    __syncwarp();
+                    if (++pbuf == C::NB) {
+                        pbuf = 0;
+                        pph ^= 1;
+                    }
+                }
+                if (++vst == NS) {
+                    vst = 0;
+                    vph ^= 1;
+                }
+            }
+        }
+        drain(ok, &bar.drain[1]);
+    } else if (warp == 10) {
+        // ---- Q rows; V rows of masked tiles ----
+        PlanWalk<RW_R, RW_KT> w(a, sc.share), wn(a, sc.share);  // the item at hand, the next one
+        constexpr int CH = C::PANELS * 8, STEP = 32 / CH;       // 16-byte pieces of a row, rows at a time
+        const int c = lane % CH;
+        const bool col = c * 8 < a.D;
+        auto load_q = [&](int item) {
+            const T *q = reinterpret_cast<const T *>(a.q) + (int64_t)wn.s.q0 * a.qs[0] + (int64_t)wn.kvh * a.G * a.qs[1] + c * 8;
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t dst = smem_u32(qs + (item % QB * 2 + t) * C::TILE) + (c / 8) * 16384;
+#pragma unroll 4
+                for (int r = lane / CH; r < 128; r += STEP) {
+                    const int f = wn.g.r0 + t * 128 + r;
+                    const bool in = f < wn.g.r1 && col;
+                    const int tok = div_g(a, f);
+                    const T *src = in ? q + (int64_t)tok * a.qs[0] + (int64_t)(f - tok * a.G) * a.qs[1]
+                                      : reinterpret_cast<const T *>(a.q);
+                    cp_async16_fill(dst + r * 128 + (((c % 8) ^ (r & 7)) << 4), src, in ? 16 : 0);
                 }
                 cp_async_commit();
-                cp_async_wait<0>();
-                fence_async_smem();
-                mbar_arrive(&bar.q_full[t]);
             }
+            cp_async_wait<0>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane < 2) mbar_arrive(&bar.q_full[item % QB * 2 + lane]);
+        };
+        int it = 0, item = 0, loaded = 0;  // key tiles and items done, items whose Q is loaded
+        bool ok = true, qmore = wn.load();
+        auto q_turn = [&](bool block) -> bool {  // the next item's Q, once its buffer is free
+            if (qtma || !qmore || loaded > item + 1) return true;
+            for (int t = 0; t < 2 && loaded >= QB; ++t) {
+                uint64_t *b = &bar.q_free[loaded % QB * 2 + t];
+                const uint32_t ph = (loaded / QB - 1) & 1;
+                if (block) {
+                    if (!wait_all(b, ph)) return false;
+                } else if (!__all_sync(0xffffffffu, mbar_test(b, ph))) {
+                    return true;
+                }
+            }
+            load_q(loaded++);
+            qmore = wn.next();
+            return true;
+        };
+        ok = q_turn(true);
+        for (bool more = w.load(); more && ok; more = w.next(), ++item) {
             for (int t = w.tl; t < w.th && ok; ++t, ++it) {
                 const int s = it % NS;
-                ok = wait(&bar.v_full[s], (it / NS) & 1);
-                if (!ok) break;
+                if (!(ok = q_turn(false)) || !(ok = wait_all(&bar.v_full[s], (it / NS) & 1))) break;
                 if (masked(w.g, t)) {
                     const int k0 = (w.g.t0 + t) * RW_KT;
+                    const KeySteps st = key_steps(w.g, t);
                     uint8_t *v = vs + s * C::TILE;
                     bool bad = false;
-                    for (int i = ht; i < 128 * C::PANELS * 8; i += 64) {
-                        const int r = (i / 8) % 128, key = k0 + r;
-                        uint4 *p = reinterpret_cast<uint4 *>(v) + i;  // 16 bytes of row r, wherever the swizzle puts them
-                        if (key < w.g.kb || key >= w.g.ke) {
-                            *p = make_uint4(0, 0, 0, 0);
-                        } else {
-                            uint4 x = *p;
-                            uint32_t *e = reinterpret_cast<uint32_t *>(&x);
+                    // rows that the products read and some row of the item does not see: before a, from b on
+                    const int a0 = max(w.g.kb, a.window > 0 ? w.g.pmax - a.window + 1 : 0) - k0, b0 = w.g.pmin + 1 - k0;
+                    const int ra = min(max(a0, st.lo * 16), st.hi * 16), rb = min(max(b0, ra), st.hi * 16);
+                    for (int r = st.lo * 16 + lane / 8; r < st.hi * 16; r += 4) {
+                        if (r >= ra && r < rb) continue;
+                        const bool out = k0 + r < w.g.kb || k0 + r >= w.g.ke;
+#pragma unroll
+                        for (int p = 0; p < C::PANELS; ++p) {
+                            uint4 *q = reinterpret_cast<uint4 *>(v + p * 16384 + r * 128) + lane % 8;
+                            if (out) {
+                                *q = make_uint4(0, 0, 0, 0);
+                                continue;
+                            }
+                            const uint4 x = *q;
+                            uint32_t e[4] = {x.x, x.y, x.z, x.w};
                             bool hit = false;
 #pragma unroll
                             for (int m = 0; m < 4; ++m) {
-                                if ((e[m] & E::EXP) == E::EXP) e[m] &= 0xFFFF0000u, hit = true;
-                                if ((e[m] >> 16 & E::EXP) == E::EXP) e[m] &= 0x0000FFFFu, hit = true;
+                                const bool lo = (e[m] & E::EXP) == E::EXP, hi = (e[m] >> 16 & E::EXP) == E::EXP;
+                                if (lo) e[m] &= 0xFFFF0000u;
+                                if (hi) e[m] &= 0x0000FFFFu;
+                                hit |= lo | hi;
                             }
-                            if (hit) {
-                                *p = x;
-                                bad = true;
-                            }
+                            if (hit) *q = make_uint4(e[0], e[1], e[2], e[3]);
+                            bad |= hit;
                         }
                     }
                     if (bad) odd[item & 3] = item + 1;
@@ -402,184 +628,256 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 }
                 mbar_arrive(&bar.v_fixed[s]);
             }
+            ok = ok && q_turn(true);
         }
     } else {
         // ---- softmax and output of row tile t ----
         const int t = warp >> 2, r = tid & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        const uint32_t sc_t = tm + lanes + C::S0 + t * 128, pt_t = tm + lanes + C::P0 + t * C::PSTEP,
-                       ot_t = tm + lanes + C::O0 + t * HD;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, ot = tm + lanes + C::O0 + t * HD;
         const float c = __fmul_rn(a.scale, 1.4426950408889634f);
+        uint8_t *ow = os + warp * 2048;
         PlanWalk<RW_R, RW_KT> w(a, sc.share);
-        int it = 0, item = 0;
+        int it = 0, item = 0;  // key tiles and items done
         uint32_t both_n = 0;
         bool ok = true;
         auto both = [&]() -> bool {  // the two row tiles' threads meet
             mbar_arrive(&bar.both);
-            return __all_sync(0xffffffffu, wait(&bar.both, both_n++ & 1));
+            return wait_all(&bar.both, both_n++ & 1);
+        };
+        // O has all products so far.  A row tile's products take two barriers
+        // in turn: a warp can be two tiles ahead of the slowest of its row
+        // tile, and the phases of one barrier would look alike to it.
+        auto o_done = [&]() -> bool {
+            const bool done = wait_all(&bar.o_full[((it - 1) & 1) * 2 + t], (it - 1) >> 1 & 1);
+            tc_fence_after();
+            return done;
         };
         for (bool more = w.load(); more && ok; more = w.next(), ++item) {
             const ItemGeo g = w.g;
-            const int f = g.r0 + t * 128 + r;
-            const int pos = f < g.r1 ? w.s.p0 + f / a.G : -1;
+            const int f = g.r0 + t * 128 + r, tok = div_g(a, f);
+            const int pos = f < g.r1 ? w.s.p0 + tok : -1;
+            const float sink = a.sinks && f < g.r1 ? __fmul_rn(a.sinks[w.kvh * a.G + f - tok * a.G], 1.4426950408889634f) : 0.0f;
             float m = -INFINITY, l = 0.0f;  // reference (of the scores as they are), sum
-            for (int j = w.tl; j < w.th && ok; ++j, ++it) {
-                ok = wait(&bar.s_full[t], it & 1);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            for (int j = w.tl; j < w.th; ++j, ++it) {
+                const int n = 2 * it + t, b = n % C::NB;
+                const uint32_t st = tm + lanes + b * 128;
+                ok = wait_all(&bar.s_full[b], (n / C::NB) & 1);
+                if (!ok) break;
                 tc_fence_after();
-                uint32_t sv[128];
+                const bool mk = masked(g, j);
+                const int hi = pos - (g.t0 + j) * RW_KT, lo = a.window > 0 ? hi - a.window : -1;  // sees lo < x <= hi
+                uint32_t sv[32];
+                float mx;
+                if (!mk) {
+                    uint32_t sw[32];
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tmem_ld32(st, sv);
+                    tmem_ld_wait32(sv);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) tmem_ld32(sc_t + 32 * x, sv + 32 * x);
-                tmem_ld_wait();
-                if (!C::ALIAS) {
-                    tc_fence_before();
-                    mbar_arrive(&bar.s_free[t]);
+                    for (int x = 0; x < 4; ++x) {  // the next 32 columns come while these are compared
+                        uint32_t *cur = x & 1 ? sw : sv, *nxt = x & 1 ? sv : sw;
+                        if (x < 3) tmem_ld32(st + 32 * x + 32, nxt);
+#pragma unroll
+                        for (int y = 0; y < 16; ++y)
+                            top[y & 3] = max3(top[y & 3], __uint_as_float(cur[2 * y]), __uint_as_float(cur[2 * y + 1]));
+                        if (x < 3) tmem_ld_wait32(nxt);
+                    }
+                    mx = max3(max3(top[0], top[1], top[2]), top[3], -INFINITY);
+                } else {
+                    mx = -INFINITY;
+#pragma unroll 1
+                    for (int x = 0; x < 128; x += 32) {
+                        const uint32_t seen = seen_bits(lo - x, hi - x);
+                        if (!__any_sync(0xffffffffu, seen != 0)) continue;
+                        tmem_ld32(st + x, sv);
+                        tmem_ld_wait32(sv);
+                        hide(sv, seen);
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
+                    }
                 }
-                if (masked(g, j)) {
-                    const int k0 = (g.t0 + j) * RW_KT, hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1;
-#pragma unroll
-                    for (int x = 0; x < 128; ++x)
-                        if (x > hi || x <= lo) sv[x] = 0xFF800000u;
-                }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int x = 0; x < 128; ++x) top[x & 3] = fmaxf(top[x & 3], __uint_as_float(sv[x]));
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 // move the reference of rows whose maximum has grown
                 const bool first = m == -INFINITY;
                 const bool grow = !first && __fmul_rn(__fsub_rn(mx, m), c) > RW_GROW;
                 float corr = 1.0f;
                 if (grow) corr = ex2(__fmul_rn(__fsub_rn(m, mx), c));
-                if (first || grow) m = mx;
+                if (first || grow || mx != mx) m = mx;
                 l = __fmul_rn(l, corr);
-                if (j > w.tl) {  // P and O are this thread's again
-                    ok = wait(&bar.o_full[t], (it - 1) & 1);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    tc_fence_after();
-                    if (__any_sync(0xffffffffu, grow)) {
+                if (__any_sync(0xffffffffu, grow)) {
+                    ok = o_done();
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int x = 0; x < HD; x += 16) {
+                        uint32_t ov[16];
+                        tmem_ld16(ot + x, ov);
+                        tmem_ld_wait16(ov);
 #pragma unroll
-                        for (int x = 0; x < HD / 16; ++x) {
-                            uint32_t ov[16];
-                            tmem_ld16(ot_t + 16 * x, ov);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) ov[y] = __float_as_uint(__fmul_rn(__uint_as_float(ov[y]), corr));
-                            tmem_st16(ot_t + 16 * x, ov);
-                        }
+                        for (int y = 0; y < 16; ++y) ov[y] = __float_as_uint(__fmul_rn(__uint_as_float(ov[y]), corr));
+                        tmem_st16(ot + x, ov);
                     }
                 }
-                const float mc = m == -INFINITY ? 0.0f : __fsub_rn(__fmul_rn(m, c), E::BIAS);
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
+                // weights 2^(s c - reference); an infinite or NaN reference makes all of them NaN
+                const float nmc = m == -INFINITY ? 0.0f : __fmaf_rn(m, 0.0f, __fsub_rn(E::BIAS, __fmul_rn(m, c)));
+                const uint64_t c2 = f2_pack(c, c), nmc2 = f2_pack(nmc, nmc);
+                uint64_t sum[2] = {0, 0};
+                tmem_ld32(st, sv);
+#pragma unroll 1
                 for (int x = 0; x < 4; ++x) {
+                    uint64_t v[16];
                     uint32_t pk[16];
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) {
-                        const float p0 = ex2(__fmaf_rn(__uint_as_float(sv[32 * x + 2 * y]), c, -mc));
-                        const float p1 = ex2(__fmaf_rn(__uint_as_float(sv[32 * x + 2 * y + 1]), c, -mc));
-                        sum[(2 * y) & 3] = __fadd_rn(sum[(2 * y) & 3], p0);
-                        sum[(2 * y + 1) & 3] = __fadd_rn(sum[(2 * y + 1) & 3], p1);
-                        pk[y] = E::pack(p0, p1);
+                    tmem_ld_wait32(sv);
+                    bool some = true, full = true;
+                    if (mk) {
+                        const uint32_t seen = seen_bits(lo - 32 * x, hi - 32 * x);
+                        some = __any_sync(0xffffffffu, seen != 0);
+                        full = __all_sync(0xffffffffu, seen == ~0u);
+                        if (some && !full) hide(sv, seen);
                     }
-                    tmem_st16(pt_t + 16 * x, pk);
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) v[y] = f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2);
+                    if (x < 3) tmem_ld32(st + 32 * x + 32, sv);
+                    if (full) {
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) {
+                            // RW_POLY of 16 pairs on the FMA units, spread among the others
+                            const uint64_t p = (y * RW_POLY) % 16 < RW_POLY ? E::pow2(v[y]) : f2_ex2(v[y]);
+                            sum[y & 1] = f2_add(sum[y & 1], p);
+                            pk[y] = E::pack(f2_lo(p), f2_hi(p));
+                        }
+                    } else if (some) {  // an unseen key's weight is 0 and nothing else
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) {
+                            const uint64_t p = f2_ex2(v[y]);
+                            sum[y & 1] = f2_add(sum[y & 1], p);
+                            pk[y] = E::pack(f2_lo(p), f2_hi(p));
+                        }
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) pk[y] = 0;
+                    }
+                    tmem_st16(st + 16 * x, pk);  // over columns read by now
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&bar.p_full[t]);
-                l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+                mbar_arrive(&bar.p_full[b]);
+                const uint64_t both_sums = f2_add(sum[0], sum[1]);
+                l = __fadd_rn(l, __fadd_rn(f2_lo(both_sums), f2_hi(both_sums)));
             }
-            if (!ok) break;
-            ok = wait(&bar.o_full[t], (it - 1) & 1);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            tc_fence_after();
-            float o[HD];
+            if (!ok || !(ok = o_done())) break;
+            float mref = m == -INFINITY ? m : __fmul_rn(m, c);  // in powers of two
+            // 32 columns of this block's O, with what masked tiles hold of non-finite V for the rows that see it
+            auto own_o = [&](int x, float (&o)[32]) {
+                uint32_t ov[32];
+                tmem_ld32(ot + x, ov);
+                tmem_ld_wait32(ov);
 #pragma unroll
-            for (int x = 0; x < HD / 32; ++x) tmem_ld32(ot_t + 32 * x, reinterpret_cast<uint32_t *>(o) + 32 * x);
-            tmem_ld_wait();
-            if (odd[item & 3] == item + 1) {  // non-finite V of masked tiles, for the rows that see it
-                for (int j = w.tl; j < w.th; ++j) {
-                    if (!masked(g, j)) continue;
-                    const int k0 = (g.t0 + j) * RW_KT;
-                    for (int key = max(max(k0, g.kb), a.window > 0 ? pos - a.window + 1 : 0);
-                         key <= min(min(k0 + RW_KT, g.ke) - 1, pos); ++key) {
-                        const T *vp = reinterpret_cast<const T *>(a.v) + (int64_t)w.kvh * a.vs[2];
-                        if (a.table) {
-                            const int page = a.table[(int64_t)w.b * a.max_pages + key / a.page_size];
-                            if (page < 0 || page >= a.n_pages) continue;
-                            vp += page * a.vs[0] + (int64_t)(key % a.page_size) * a.vs[1];
-                        } else {
-                            vp += (int64_t)(w.s.q0 + key) * a.vs[1];
-                        }
+                for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(ov[d]);
+                if (odd[item & 3] != item + 1) return;
+                const T *vb = reinterpret_cast<const T *>(a.v) + (int64_t)w.kvh * a.vs[2];
+                for (int key = (g.t0 + w.tl) * RW_KT; key < (g.t0 + w.th) * RW_KT; ++key) {
+                    if (key < g.kb || key >= g.ke || key > pos || (a.window > 0 && key <= pos - a.window) ||
+                        !masked(g, key / RW_KT - g.t0))
+                        continue;
+                    const T *vp = vb + (int64_t)(w.s.q0 + key) * a.vs[1];
+                    if (a.table) {
+                        const int page = a.table[(int64_t)w.b * a.max_pages + key / a.page_size];
+                        if (page < 0 || page >= a.n_pages) continue;
+                        vp = vb + page * a.vs[0] + (int64_t)(key % a.page_size) * a.vs[1];
+                    }
 #pragma unroll
-                        for (int d = 0; d < HD; ++d)
-                            if (d < a.D) {
-                                const float v = E::up(reinterpret_cast<const unsigned short *>(vp)[d]);
-                                if (!isfinite(v)) o[d] = __fadd_rn(o[d], v);
-                            }
+                    for (int d = 0; d < 32; ++d) {
+                        const float v = x + d < a.D ? E::up(reinterpret_cast<const unsigned short *>(vp)[x + d]) : 0.0f;
+                        if (!isfinite(v)) o[d] = __fadd_rn(o[d], v);
                     }
                 }
-            }
-            float mref = m == -INFINITY ? m : __fmul_rn(m, c);  // in powers of two
-            if (!w.whole()) {
-                const CutItem cut = cut_item(w);
-                float *mine = a.part + ((int64_t)blockIdx.x * 2 + (w.tl == 0)) * C::PART;
+            };
+            const bool cut = !w.whole();
+            CutItem ci = {0, 0};
+            if (cut) {
+                ci = cut_item(w);
+                float *mine = a.part + ((int64_t)blockIdx.x * 2 + (w.tl == 0)) * C::PART + tid;
+#pragma unroll 1
+                for (int x = 0; x < HD; x += 32) {
+                    float o[32];
+                    own_o(x, o);
 #pragma unroll
-                for (int d = 0; d < HD; ++d) __stcg(mine + d * RW_R + tid, o[d]);
-                __stcg(mine + HD * RW_R + tid, mref);
-                __stcg(mine + (HD + 1) * RW_R + tid, l);
+                    for (int d = 0; d < 32; ++d) __stcg(mine + (x + d) * RW_R, o[d]);
+                }
+                __stcg(mine + HD * RW_R, mref);
+                __stcg(mine + (HD + 1) * RW_R, l);
                 __threadfence();
                 if (!(ok = both())) break;
                 if (tid == 0) {
-                    lastf = atomicAdd(a.ticket + cut.k0, 1u) == (unsigned)(cut.k1 - cut.k0);
-                    if (lastf) a.ticket[cut.k0] = 0u;
+                    lastf = atomicAdd(a.ticket + ci.k0, 1u) == (unsigned)(ci.k1 - ci.k0);
+                    if (lastf) a.ticket[ci.k0] = 0u;
                 }
                 if (!(ok = both())) break;
                 if (!lastf) continue;
                 __threadfence();
                 float mm = -INFINITY;
-                for (int k = cut.k0; k <= cut.k1; ++k)
-                    mm = fmaxf(mm, __ldcg(a.part + ((int64_t)k * 2 + (k == cut.k0)) * C::PART + HD * RW_R + tid));
+                for (int k = ci.k0; k <= ci.k1; ++k)
+                    mm = fmaxf(mm, __ldcg(a.part + ((int64_t)k * 2 + (k == ci.k0)) * C::PART + HD * RW_R + tid));
                 const float ms = mm == -INFINITY ? 0.0f : mm;
                 l = 0.0f;
-#pragma unroll
-                for (int d = 0; d < HD; ++d) o[d] = 0.0f;
-                for (int k = cut.k0; k <= cut.k1; ++k) {
-                    const float *p = a.part + ((int64_t)k * 2 + (k == cut.k0)) * C::PART + tid;
-                    const float e = ex2(__fsub_rn(__ldcg(p + HD * RW_R), ms));
-                    l = __fmaf_rn(__ldcg(p + (HD + 1) * RW_R), e, l);
-#pragma unroll
-                    for (int d = 0; d < HD; ++d) o[d] = __fmaf_rn(__ldcg(p + d * RW_R), e, o[d]);
+                for (int k = ci.k0; k <= ci.k1; ++k) {
+                    const float *p = a.part + ((int64_t)k * 2 + (k == ci.k0)) * C::PART + HD * RW_R + tid;
+                    l = __fmaf_rn(__ldcg(p + RW_R), ex2(__fsub_rn(__ldcg(p), ms)), l);
                 }
                 mref = mm;
             }
-            if (f < g.r1) {
-                const int h = w.kvh * a.G + f % a.G;
-                const bool none = mref == -INFINITY && l == 0.0f;  // no key seen
-                float inv = 0.0f;
-                if (!none) {
-                    float den = l;
-                    if (a.sinks) {
-                        // both on the larger of the two references; E::BIAS is in l and o
-                        const float sk = __fmul_rn(a.sinks[h], 1.4426950408889634f), mm = fmaxf(mref, sk);
-                        const float e = ex2(__fsub_rn(mref, mm));
-                        den = __fmaf_rn(l, e, ex2(__fadd_rn(__fsub_rn(sk, mm), E::BIAS)));
-                        inv = __fdiv_rn(e, den);
-                    } else {
-                        inv = __fdiv_rn(1.0f, den);
+            const bool none = mref == -INFINITY && l == 0.0f;  // no key seen
+            float inv = 0.0f;
+            if (!none && f < g.r1) {
+                if (a.sinks) {
+                    // both on the larger of the two references; E::BIAS is in l and o
+                    const float mm = fmaxf(mref, sink), e = ex2(__fsub_rn(mref, mm));
+                    inv = __fdividef(e, __fmaf_rn(l, e, ex2(__fadd_rn(__fsub_rn(sink, mm), E::BIAS))));
+                } else {
+                    inv = __fdividef(1.0f, l);
+                }
+            }
+            // through shared memory, so that four lanes write 64 bytes of a row
+#pragma unroll 1
+            for (int x = 0; x < HD; x += 32) {
+                float o[32];
+                if (!cut) {
+                    own_o(x, o);
+                } else {
+                    const float ms = mref == -INFINITY ? 0.0f : mref;
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) o[d] = 0.0f;
+#pragma unroll 1
+                    for (int k = ci.k0; k <= ci.k1; ++k) {
+                        const float *p = a.part + ((int64_t)k * 2 + (k == ci.k0)) * C::PART + tid;
+                        const float e = ex2(__fsub_rn(__ldcg(p + HD * RW_R), ms));
+#pragma unroll
+                        for (int d = 0; d < 32; ++d) o[d] = __fmaf_rn(__ldcg(p + (x + d) * RW_R), e, o[d]);
                     }
                 }
-                T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.s.q0 + f / a.G) * a.os[0] + (int64_t)h * a.os[1];
+                __syncwarp();
 #pragma unroll
-                for (int d = 0; d < HD; d += 8)
-                    if (d < a.D) {
-                        uint4 v;
-                        uint32_t *e = reinterpret_cast<uint32_t *>(&v);
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint32_t e[4];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y)
-                            e[y] = none ? 0u : E::pack(__fmul_rn(o[d + 2 * y], inv), __fmul_rn(o[d + 2 * y + 1], inv));
-                        *reinterpret_cast<uint4 *>(out + d) = v;
+                    for (int y = 0; y < 4; ++y)
+                        e[y] = none ? 0u : E::pack(__fmul_rn(o[ch * 8 + 2 * y], inv), __fmul_rn(o[ch * 8 + 2 * y + 1], inv));
+                    *reinterpret_cast<uint4 *>(ow + lane * 64 + ((ch ^ (lane >> 1 & 3)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+                }
+                __syncwarp();
+                const int ch = lane & 3;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int rr = 8 * i + (lane >> 2), ff = g.r0 + t * 128 + (warp & 3) * 32 + rr;
+                    if (ff < g.r1 && x + ch * 8 < a.D) {
+                        const int ft = div_g(a, ff);
+                        T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.s.q0 + ft) * a.os[0] +
+                                 (int64_t)(w.kvh * a.G + ff - ft * a.G) * a.os[1] + x + ch * 8;
+                        *reinterpret_cast<uint4 *>(out) =
+                            *reinterpret_cast<const uint4 *>(ow + rr * 64 + ((ch ^ (rr >> 1 & 3)) << 4));
                     }
+                }
             }
+            tc_fence_before();
         }
     }
     tc_fence_before();
@@ -614,8 +912,9 @@ cudaError_t rows_set() {
 }
 
 template <typename T, int HD>
-cudaError_t rows_run(const AttnOp &a, const CUtensorMap &k, const CUtensorMap &v, int box, int nsm, cudaStream_t st) {
-    return launch_k(attn_rows_kernel<T, HD>, dim3(nsm), dim3(RW_THREADS), RowsCfg<HD>::SMEM, st, a, k, v, box);
+cudaError_t rows_run(const AttnOp &a, const CUtensorMap &k, const CUtensorMap &v, const CUtensorMap &q, int box,
+                     bool qtma, int nsm, cudaStream_t st) {
+    return launch_k(attn_rows_kernel<T, HD>, dim3(nsm), dim3(RW_THREADS), RowsCfg<HD>::SMEM, st, a, k, v, q, box, qtma);
 }
 
 }  // namespace
@@ -650,16 +949,34 @@ cudaError_t attn_rows_configure() {
     return e;
 }
 
+// Q as a tensor map whose box is a row tile: 128 / G tokens x G heads x 64
+// columns (G divides 128); false if there is none.
+bool q_tensor_map(const AttnOp &a, int dtype, CUtensorMap &m) {
+    EncodeTiledFn fn = rows_encode_fn();
+    if (!fn || 128 % a.G) return false;
+    const cuuint64_t unit = (cuuint64_t)((a.D * 2 + 15) / 16 * 16);
+    const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.H, (cuuint64_t)a.T};
+    const cuuint64_t strides[2] = {a.H == 1 ? unit : (cuuint64_t)a.qs[1] * 2, a.T == 1 ? unit : (cuuint64_t)a.qs[0] * 2};
+    const cuuint32_t boxes[3] = {64u, (cuuint32_t)a.G, (cuuint32_t)(128 / a.G)}, es[3] = {1u, 1u, 1u};
+    return fn(&m, dtype == PC_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+              const_cast<void *>(a.q), dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool launch_attn_rows(const AttnOp &a, int dtype, int nsm, cudaStream_t st, cudaError_t &e) {
     // positions per TMA box: the largest power of two that divides a page
-    const int box = a.table ? min(a.page_size & -a.page_size, RW_KT) : RW_KT;
-    CUtensorMap k, v;
+    const int box = a.table ? std::min(a.page_size & -a.page_size, RW_KT) : RW_KT;
+    CUtensorMap k, v, q;
     if (!kv_tensor_map(a, false, dtype, box, k) || !kv_tensor_map(a, true, dtype, box, v)) return false;
+    const bool qtma = q_tensor_map(a, dtype, q);
+    if (!qtma) q = k;  // not read
     if (dtype == PC_DT_F16)
-        e = a.D <= 64 ? rows_run<__half, 64>(a, k, v, box, nsm, st) : rows_run<__half, 128>(a, k, v, box, nsm, st);
+        e = a.D <= 64 ? rows_run<__half, 64>(a, k, v, q, box, qtma, nsm, st)
+                      : rows_run<__half, 128>(a, k, v, q, box, qtma, nsm, st);
     else
-        e = a.D <= 64 ? rows_run<__nv_bfloat16, 64>(a, k, v, box, nsm, st)
-                      : rows_run<__nv_bfloat16, 128>(a, k, v, box, nsm, st);
+        e = a.D <= 64 ? rows_run<__nv_bfloat16, 64>(a, k, v, q, box, qtma, nsm, st)
+                      : rows_run<__nv_bfloat16, 128>(a, k, v, q, box, qtma, nsm, st);
     return true;
 }
 

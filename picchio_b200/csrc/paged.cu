@@ -70,7 +70,8 @@ pc_status check_call(const pc_attn_call *c) {
     if (!dt_ok(c->dtype)) return fail(PC_ERR_FORMAT, "type must be PC_DT_F32, PC_DT_F16 or PC_DT_BF16");
     if (c->head_dim < 8 || c->head_dim > 128 || c->head_dim % 8)
         return fail(PC_ERR_FORMAT, "head_dim must be a multiple of 8, at most 128");
-    if (c->n_rows > (1 << 24) / (c->n_heads / c->n_kv_heads) * 8 || c->n_requests > (1 << 24))
+    const int64_t group = c->n_heads / c->n_kv_heads;
+    if (c->n_rows * group * group >= (1ll << 32) || c->n_rows * group > (1 << 27) || c->n_requests > (1 << 24))
         return fail(PC_ERR_RANGE, "too many rows or requests");
     if (c->n_rows == 0 || c->n_requests == 0) return PC_OK;
     if (!c->q_dev || !c->out_dev || !c->cu_new_dev) return fail(PC_ERR_INVALID_ARG, "null tensor");
@@ -97,6 +98,7 @@ AttnOp op_of(const pc_attn *a, const pc_attn_call *c) {
     o.KVH = c->n_kv_heads;
     o.G = c->n_heads / c->n_kv_heads;
     o.D = c->head_dim;
+    o.inv_g = (unsigned)(((1ull << 32) + o.G - 1) / o.G);
     o.window = c->window;
     o.scale = c->scale;
     o.min_q = 1;

@@ -21,6 +21,7 @@ struct AttnOp {
     int max_pages, page_size, n_pages;
     int B, T, H, KVH, G, D, window;
     float scale;
+    unsigned inv_g;        // 2^32 / G rounded up (G > 1)
     int min_q, max_q;      // the kernel takes requests with min_q <= rows * G <= max_q
     float *part;           // partial (O, m, l) of items cut between CTAs, two slots per CTA
     unsigned *ticket;      // one per CTA, zero between calls
