@@ -55,7 +55,7 @@ namespace pc {
 
 namespace {
 
-constexpr int RW_R = 256, RW_KT = 128, RW_OV = 128, RW_MINK = 256, RW_THREADS = 384;
+constexpr int RW_R = 256, RW_KT = 128, RW_OV = 384, RW_MINK = 256, RW_THREADS = 384;
 constexpr long long RW_WAIT_CLOCKS = 2000000000ll;  // about a second
 constexpr float RW_GROW = 8.0f;                     // log2 of the growth that moves the reference
 
