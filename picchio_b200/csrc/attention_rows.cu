@@ -42,21 +42,16 @@
 // pages) are zeroed and non-finite V elements of the others taken out before
 // the product; if there were any, the rows that see them get them added back
 // from global memory at the end of the item.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
-#include "attention_plan.cuh"
+#include "attention_half.cuh"
 #include "launch.cuh"
-#include "sm100.cuh"
 
 namespace pc {
 
 namespace {
 
 constexpr int RW_R = 256, RW_KT = 128, RW_OV = 384, RW_MINK = 256, RW_THREADS = 384;
-constexpr long long RW_WAIT_CLOCKS = 2000000000ll;  // about a second
 constexpr float RW_GROW = 8.0f;                     // log2 of the growth that moves the reference
 
 template <int HD>
@@ -80,21 +75,6 @@ struct RowsBars {
     uint64_t k_full[3], k_free[3], v_full[3], v_free[3], v_fixed[3], both, drain[2];
 };
 
-__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z,
-                                            int w) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-        "%5}], [%6];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-        : "memory");
-}
 __device__ __forceinline__ void cp_async16_fill(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -155,26 +135,6 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
 __device__ __forceinline__ uint64_t sw128_desc_n(uint32_t saddr, int panel) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(panel >> 4) << 16) | ((1024ull >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// mbar_try_wait that may sleep up to 20 us: a waiting warp issues nothing
-// that the row warps of its scheduler would have to wait for
-__device__ __forceinline__ bool mbar_sleep_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
 }
 
 // Whether a phase is complete, without waiting
@@ -256,37 +216,18 @@ __device__ __forceinline__ uint64_t f2_pow2(uint64_t x, const float (&c)[DEG + 1
     return f2_pack_bits((uint32_t)p + ((uint32_t)t << 23), (uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23));
 }
 
-// Element types: instruction-descriptor code, packing, the bits of a
-// non-finite exponent, and the power of two that weights are stored at (f16
-// weights keep 7 binary orders more before they underflow; the sums carry
-// the same factor, so the quotient does not change).
+// What part of the exponentials runs as f2_pow2 with, by the weights' type
 template <typename T>
-struct Half16;
+struct Pow2;
 template <>
-struct Half16<__nv_bfloat16> {
-    static constexpr uint32_t FMT = 1, EXP = 0x7F80u;
-    static constexpr float BIAS = 0.0f;
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        uint32_t r;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-        return r;
-    }
-    static __device__ __forceinline__ float up(uint32_t h) { return __uint_as_float(h << 16); }
-    static __device__ __forceinline__ uint64_t pow2(uint64_t x) {
+struct Pow2<__nv_bfloat16> {
+    static __device__ __forceinline__ uint64_t of(uint64_t x) {
         return f2_pow2<3>(x, {0.9999280571937561f, 0.6932609677314758f, 0.2426111251115799f, 0.0551716685295105f});
     }
 };
 template <>
-struct Half16<__half> {
-    static constexpr uint32_t FMT = 0, EXP = 0x7C00u;
-    static constexpr float BIAS = 7.0f;
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        uint32_t r;
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-        return r;
-    }
-    static __device__ __forceinline__ float up(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)h)); }
-    static __device__ __forceinline__ uint64_t pow2(uint64_t x) {
+struct Pow2<__half> {
+    static __device__ __forceinline__ uint64_t of(uint64_t x) {
         return f2_pow2<4>(x, {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f, 0.05591785907745361f,
                               0.009570102207362652f});
     }
@@ -346,20 +287,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
     tc_fence_after();
     const uint32_t tm = tmem_slot;
 
-    // A bounded wait: false once it, or any other wait of the block, gave up.
-    auto wait = [&](uint64_t *b, uint32_t parity) -> bool {
-        if (mbar_sleep_wait(b, parity)) return true;
-        const long long t0 = clock64();
-        while (!mbar_sleep_wait(b, parity)) {
-            if (dead) return false;
-            if (clock64() - t0 > RW_WAIT_CLOCKS) {
-                dead = 1;
-                atomicExch(a.err, 1);
-                return false;
-            }
-        }
-        return true;
-    };
+    auto wait = [&](uint64_t *b, uint32_t parity) -> bool { return bounded_wait(b, parity, &dead, a.err); };
     auto wait_all = [&](uint64_t *b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
     // the steps of 16 keys of a tile that hold keys of the item (one at least)
     auto key_steps = [&](const ItemGeo &g, int t) -> KeySteps {
@@ -375,7 +303,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             tc_commit(b);
             const long long t0 = clock64();
             while (!mbar_try_wait(b, 0))
-                if (clock64() - t0 > RW_WAIT_CLOCKS) break;
+                if (clock64() - t0 > ATTN_WAIT_CLOCKS) break;
         }
         __syncwarp();
     };
@@ -449,7 +377,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                     const long long t0 = clock64();
                     if (n > 0)
                         while (!mbar_try_wait(kv ? &bar.v_full[s] : &bar.k_full[s], (n - 1) & 1))
-                            if (clock64() - t0 > RW_WAIT_CLOCKS) break;
+                            if (clock64() - t0 > ATTN_WAIT_CLOCKS) break;
                 }
     } else if (warp == 9) {
         // ---- S = Q K^T ----
@@ -740,7 +668,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
 #pragma unroll
                         for (int y = 0; y < 16; ++y) {
                             // RW_POLY of 16 pairs on the FMA units, spread among the others
-                            const uint64_t p = (y * RW_POLY) % 16 < RW_POLY ? E::pow2(v[y]) : f2_ex2(v[y]);
+                            const uint64_t p = (y * RW_POLY) % 16 < RW_POLY ? Pow2<T>::of(v[y]) : f2_ex2(v[y]);
                             sum[y & 1] = f2_add(sum[y & 1], p);
                             pk[y] = E::pack(f2_lo(p), f2_hi(p));
                         }
@@ -826,16 +754,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 mref = mm;
             }
             const bool none = mref == -INFINITY && l == 0.0f;  // no key seen
-            float inv = 0.0f;
-            if (!none && f < g.r1) {
-                if (a.sinks) {
-                    // both on the larger of the two references; E::BIAS is in l and o
-                    const float mm = fmaxf(mref, sink), e = ex2(__fsub_rn(mref, mm));
-                    inv = __fdividef(e, __fmaf_rn(l, e, ex2(__fadd_rn(__fsub_rn(sink, mm), E::BIAS))));
-                } else {
-                    inv = __fdividef(1.0f, l);
-                }
-            }
+            const float inv = f < g.r1 ? row_factor<E>(mref, l, a.sinks != nullptr, sink) : 0.0f;
             // through shared memory, so that four lanes write 64 bytes of a row
 #pragma unroll 1
             for (int x = 0; x < HD; x += 32) {
@@ -919,9 +838,6 @@ cudaError_t rows_run(const AttnOp &a, const CUtensorMap &k, const CUtensorMap &v
 
 }  // namespace
 
-// K or V as a tensor map: rows of head_dim elements, boxes of 64 columns x
-// `box` positions of one head, 128-byte swizzle, zeros outside.  False if its
-// strides cannot be described (a stride of zero).
 bool kv_tensor_map(const AttnOp &a, bool v, int dtype, int box, CUtensorMap &m) {
     EncodeTiledFn fn = rows_encode_fn();
     if (!fn) return false;

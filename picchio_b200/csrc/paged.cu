@@ -109,10 +109,38 @@ AttnOp op_of(const pc_attn *a, const pc_attn_call *c) {
     return o;
 }
 
+// f16 and bf16 have two kernels: one for few rows of a request and KV head
+// (tokens x query heads of the group), bound by reading K and V, and one for
+// many, bound by the products.  Which a request takes goes by its own rows,
+// read on the device; where the batch has no more rows than the first takes
+// of each request, the second is not launched (a request of more rows then
+// takes the first in several passes), and over whole prompts the first is not.
+constexpr int FEW_ROWS = 16;
+
 pc_status run_attention(pc_attn *a, const AttnOp &o, int dtype, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
-    if (dtype == PC_DT_F32 || !launch_attn_rows(o, dtype, a->nsm, st, e)) e = launch_attn_simt(o, dtype, a->nsm, st);
-    PC_CU(e);
+    if (dtype != PC_DT_F32) {
+        if (!o.table) {
+            if (launch_attn_rows(o, dtype, a->nsm, st, e)) {
+                PC_CU(e);
+                return PC_OK;
+            }
+        } else {
+            AttnOp few = o, many = o;
+            const bool all_few = (int64_t)o.T * o.G <= (int64_t)std::max(o.G, FEW_ROWS) * o.B;
+            if (!all_few) {
+                few.max_q = std::max(o.G, FEW_ROWS);
+                many.min_q = few.max_q + 1;
+            }
+            if (launch_attn_few(few, dtype, a->nsm, st, e)) {
+                if (e == cudaSuccess && !all_few && !launch_attn_rows(many, dtype, a->nsm, st, e))
+                    e = launch_attn_simt(many, dtype, a->nsm, st);
+                PC_CU(e);
+                return PC_OK;
+            }
+        }
+    }
+    PC_CU(launch_attn_simt(o, dtype, a->nsm, st));
     return PC_OK;
 }
 
@@ -172,7 +200,8 @@ pc_status pc_attn_create(int device, pc_attn **out) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&a->max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
     if (e == cudaSuccess) e = attn_simt_configure();
     if (e == cudaSuccess) e = attn_rows_configure();
-    const size_t part = std::max(attn_simt_part_floats(a->nsm), attn_rows_part_floats(a->nsm));
+    if (e == cudaSuccess) e = attn_few_configure();
+    const size_t part = std::max({attn_simt_part_floats(a->nsm), attn_rows_part_floats(a->nsm), attn_few_part_floats(a->nsm)});
     if (e == cudaSuccess) e = cudaMalloc(&a->part, part * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&a->ticket, ATTN_MAX_CTAS * sizeof(unsigned));
     if (e == cudaSuccess) e = cudaMalloc(&a->err, sizeof(int));

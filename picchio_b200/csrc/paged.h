@@ -41,6 +41,11 @@ size_t attn_rows_part_floats(int nsm);
 cudaError_t attn_rows_configure();
 bool launch_attn_rows(const AttnOp &a, int dtype, int nsm, cudaStream_t st, cudaError_t &e);
 
+// The same for few rows a request.
+size_t attn_few_part_floats(int nsm);
+cudaError_t attn_few_configure();
+bool launch_attn_few(const AttnOp &a, int dtype, int nsm, cudaStream_t st, cudaError_t &e);
+
 cudaError_t launch_kv_tables(const pc_kv_step &s, cudaStream_t st);
 cudaError_t launch_kv_store(const pc_kv_pages &kv, const void *k, const int64_t *ks, const void *v, const int64_t *vs,
                             int src_dtype, const int64_t *slot, int n, int nsm, cudaStream_t st);

@@ -187,6 +187,15 @@ def test_paged_long_rows_are_split(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 32)])
+def test_paged_many_tiles_a_block(dtype, D, page):
+    """Each block goes through its ring of tiles many times, and from item to
+    item, with warps ahead of one another."""
+    check_paged([(2900 + 37 * (i % 11), 1) for i in range(48)], page, 32, 4, D, dtype, True, 0)
+    check_paged([(2500 + 91 * (i % 7), 1 + 60 * (i % 4 == 3)) for i in range(24)], page, 32, 8, D, dtype, False, 700)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_rows_without_keys_give_zeros(dtype):
     """Fewer positions in the cache than new rows: the first rows stand before
     position 0 and see nothing, with and without sinks."""
