@@ -44,26 +44,63 @@ __device__ __forceinline__ void block_scan3(int (&v)[3], int (&all)[3], int (*sh
     }
 }
 
-// One block: the requests in chunks of 1024, each chunk a scan.
+// Position and slot of the step's row t: its request by bisection of cu_new.
+__device__ __forceinline__ void row_slot(const pc_kv_step &s, int t, int total) {
+    if (t >= total) {
+        s.pos_dev[t] = -1;
+        s.slot_dev[t] = -1;
+        return;
+    }
+    int lo = 0, hi = s.n_requests;  // cu_new[lo] <= t < cu_new[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s.cu_new_dev[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    const int p = max(s.kv_len_dev[lo], 0) + t - s.cu_new_dev[lo], page = p / s.page_size;
+    s.pos_dev[t] = p;
+    s.slot_dev[t] = (int64_t)s.page_table_dev[(int64_t)lo * s.max_pages + page] * s.page_size + p % s.page_size;
+}
+
+// Up to how many rows the table block fills in itself, one a thread; more
+// rows have a launch of their own, which is 2 us more for the smallest steps
+// and saves 40 us at 16,000 rows.
+constexpr int TAB_ROWS = TAB_THREADS;
+
+// One block: the requests in chunks of 1024, each chunk a scan; a request's
+// pages are moved by its thread if they are one or two, else by its warp.
+// Bound by latency: a few dependent trips to L2 and the scans' barriers.
 __global__ void __launch_bounds__(TAB_THREADS) kv_tables_kernel(const pc_kv_step s) {
     __shared__ int sh[3][TAB_THREADS / 32];
-    const int tid = threadIdx.x, P = s.page_size;
+    const int tid = threadIdx.x, lane = tid & 31, P = s.page_size;
     pdl_wait();
     pdl_trigger();
     const int n_free = min(max(*s.n_free_dev, 0), s.free_cap);
+    // `move(b, j, at)` for the n things of request b that go to `at` on
+    auto each = [&](int b, int n, int at, auto move) {
+        if (n <= 2)
+            for (int j = 0; j < n; ++j) move(b, j, at + j);
+        for (unsigned more = __ballot_sync(0xffffffffu, n > 2); more; more &= more - 1) {
+            const int src = __ffs(more) - 1;
+            const int bb = __shfl_sync(0xffffffffu, b, src), nn = __shfl_sync(0xffffffffu, n, src),
+                      aa = __shfl_sync(0xffffffffu, at, src);
+            for (int j = lane; j < nn; j += 32) move(bb, j, aa + j);
+        }
+    };
     // pages of ended requests on top of the free ones
     int given = 0;
     for (int b0 = 0; b0 < s.n_requests; b0 += TAB_THREADS) {
         const int b = b0 + tid;
         int v[3] = {0, 0, 0}, all[3];
         if (b < s.n_requests && s.new_len_dev[b] < 0)
-            v[0] = min((max(s.kv_len_dev[b], 0) + P - 1) / P, s.max_pages);
+            v[0] = min((int)(((int64_t)max(s.kv_len_dev[b], 0) + P - 1) / P), s.max_pages);
         const int n = v[0];
+        if (!__syncthreads_or(n)) continue;
         block_scan3(v, all, sh);
-        const int at = n_free + given + v[0] - n;
-        for (int j = 0; j < n; ++j)
-            if (at + j < s.free_cap) s.free_pages_dev[at + j] = s.page_table_dev[(int64_t)b * s.max_pages + j];
-        given += all[0];
+        each(b, n, n_free + given + v[0] - n, [&](int r, int j, int at) {
+            if (at < s.free_cap) s.free_pages_dev[at] = s.page_table_dev[(int64_t)r * s.max_pages + j];
+        });
+        given = (int)min((int64_t)given + all[0], (int64_t)1 << 30);
     }
     const int avail = min(n_free + given, s.free_cap);
     __syncthreads();
@@ -78,7 +115,7 @@ __global__ void __launch_bounds__(TAB_THREADS) kv_tables_kernel(const pc_kv_step
             add = s.new_len_dev[b];
             ended = add < 0;
             fits = !ended && (int64_t)kv + add <= (int64_t)s.max_pages * P;
-            held = (kv + P - 1) / P;
+            held = fits ? (kv + P - 1) / P : 0;
             v[0] = fits ? (kv + add + P - 1) / P - held : 0;
             v[1] = fits ? min(add, s.n_tokens + 1) : 0;
         }
@@ -88,33 +125,36 @@ __global__ void __launch_bounds__(TAB_THREADS) kv_tables_kernel(const pc_kv_step
         const bool ok = fits && (want == 0 || upto <= avail) && (add == 0 || tokens <= s.n_tokens);
         int u[3] = {ok ? add : 0, ok ? want : 0, 0}, uall[3];
         block_scan3(u, uall, sh);
+        // request b's page held + j is the (upto - want + j)-th from the top of the free ones
+        const int first = ok && want ? (int)(upto - want) : 0;
+        each(b, ok ? want : 0, first, [&](int r, int j, int nth) {
+            const int kept = (max(s.kv_len_dev[r], 0) + P - 1) / P;
+            s.page_table_dev[(int64_t)r * s.max_pages + kept + j] = s.free_pages_dev[avail - 1 - nth];
+        });
         if (b < s.n_requests) {
-            int *row = s.page_table_dev + (int64_t)b * s.max_pages;
-            if (ok)
-                for (int j = 0; j < want; ++j) row[held + j] = s.free_pages_dev[avail - 1 - (int)(upto - want) - j];
             s.kv_end_dev[b] = ended ? 0 : ok ? kv + add : kv;
             s.served_dev[b] = ok;
             s.cu_new_dev[b + 1] = took0 + u[0];
-            if (ok)
-                for (int i = 0; i < add; ++i) {
-                    const int p = kv + i, t = took0 + u[0] - add + i;
-                    s.pos_dev[t] = p;
-                    s.slot_dev[t] = (int64_t)row[p / P] * P + p % P;
-                }
         }
         want0 = (int)min((int64_t)want0 + all[0], (int64_t)1 << 30);
         add0 = (int)min((int64_t)add0 + all[1], (int64_t)1 << 30);
         took0 += uall[0];
         used += uall[1];
     }
-    for (int t = took0 + tid; t < s.n_tokens; t += TAB_THREADS) {
-        s.pos_dev[t] = -1;
-        s.slot_dev[t] = -1;
-    }
     if (tid == 0) {
         s.cu_new_dev[0] = 0;
         *s.n_free_out_dev = avail - used;
     }
+    if (s.n_tokens > TAB_ROWS) return;
+    __syncthreads();
+    if (tid < s.n_tokens) row_slot(s, tid, took0);
+}
+
+__global__ void __launch_bounds__(256) kv_slots_kernel(const pc_kv_step s) {
+    pdl_wait();
+    pdl_trigger();
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t < s.n_tokens) row_slot(s, t, s.cu_new_dev[s.n_requests]);
 }
 
 struct StoreOp {
@@ -134,49 +174,88 @@ template <> __device__ __forceinline__ float down<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half down<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 down<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// 8 elements as loaded and stored: 16 or 32 bytes
 template <typename T>
-struct alignas(sizeof(T) * 8) Vec8 {
-    T v[8];
-};
+__device__ __forceinline__ void load8(const T *p, float (&f)[8]) {
+    uint4 r[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    const T *t = reinterpret_cast<const T *>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = up(t[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const float (&f)[8]) {
+    uint4 r[sizeof(T) / 2];
+    T *t = reinterpret_cast<T *>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = down<T>(f[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = r[i];
+}
 
-// A thread moves 8 elements of a K row and the same of the V row.
+// A block takes `rows` rows of the step, a thread 8 elements of K and the same
+// of V at a time.  Bytes only: 16-byte loads and stores, all of a thread's
+// loads before its stores.
+constexpr int ST_UNROLL = 2;
 template <typename S, typename D>
-__global__ void __launch_bounds__(256) kv_store_kernel(const StoreOp o) {
+__global__ void __launch_bounds__(256) kv_store_kernel(const StoreOp o, const int rows) {
     pdl_wait();
     pdl_trigger();
     const int per = o.D / 8, row = o.KVH * per;
-    const int64_t n = (int64_t)o.n * row;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int t = (int)(i / row), c = (int)(i % row), h = c / per, d = (c % per) * 8;
-        const int64_t slot = o.slot[t];
-        if (slot < 0 || slot >= o.slots) continue;
-        const int64_t page = slot / o.page, r = slot % o.page;
+    const int64_t t0 = (int64_t)blockIdx.x * rows;
+    const int n = (int)min((int64_t)rows, o.n - t0) * row;
+    for (int i0 = threadIdx.x; i0 < n; i0 += 256 * ST_UNROLL) {
+        float k[ST_UNROLL][8], v[ST_UNROLL][8];
+        int64_t kd[ST_UNROLL], vd[ST_UNROLL];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const S *src = reinterpret_cast<const S *>(w ? o.v : o.k) + t * (w ? o.vs : o.ks)[0] +
-                           h * (w ? o.vs : o.ks)[1] + d;
-            const int64_t *cs = w ? o.vcs : o.kcs;
-            D *dst = reinterpret_cast<D *>(w ? o.vc : o.kc) + page * cs[0] + r * cs[1] + h * cs[2] + d;
-            D y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = down<D>(up(src[j]));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dst[j] = y[j];
+        for (int u = 0; u < ST_UNROLL; ++u) {
+            const int i = i0 + 256 * u;
+            kd[u] = -1;
+            if (i >= n) continue;
+            const int r = i / row, c = i - r * row, h = c / per, d = (c - h * per) * 8;
+            const int64_t t = t0 + r, slot = o.slot[t];
+            if (slot < 0 || slot >= o.slots) continue;
+            int64_t page, at;
+            if (slot >> 31 == 0) {
+                page = (unsigned)slot / (unsigned)o.page;
+                at = (unsigned)slot - (unsigned)page * (unsigned)o.page;
+            } else {
+                page = slot / o.page;
+                at = slot - page * o.page;
+            }
+            kd[u] = page * o.kcs[0] + at * o.kcs[1] + h * o.kcs[2] + d;
+            vd[u] = page * o.vcs[0] + at * o.vcs[1] + h * o.vcs[2] + d;
+            load8(reinterpret_cast<const S *>(o.k) + t * o.ks[0] + h * o.ks[1] + d, k[u]);
+            load8(reinterpret_cast<const S *>(o.v) + t * o.vs[0] + h * o.vs[1] + d, v[u]);
         }
+#pragma unroll
+        for (int u = 0; u < ST_UNROLL; ++u)
+            if (kd[u] >= 0) {
+                store8(reinterpret_cast<D *>(o.kc) + kd[u], k[u]);
+                store8(reinterpret_cast<D *>(o.vc) + vd[u], v[u]);
+            }
     }
 }
 
 template <typename S>
-cudaError_t store_to(const StoreOp &o, int dtype, int grid, cudaStream_t st) {
-    if (dtype == PC_DT_F32) return launch_k(kv_store_kernel<S, float>, dim3(grid), dim3(256), 0, st, o);
-    if (dtype == PC_DT_F16) return launch_k(kv_store_kernel<S, __half>, dim3(grid), dim3(256), 0, st, o);
-    return launch_k(kv_store_kernel<S, __nv_bfloat16>, dim3(grid), dim3(256), 0, st, o);
+cudaError_t store_to(const StoreOp &o, int dtype, int nsm, cudaStream_t st) {
+    // rows a block: two pieces a thread, fewer while that leaves SMs without a block
+    const int row = o.KVH * (o.D / 8);
+    int rows = std::max(1, 256 * ST_UNROLL / row);
+    while (rows > 1 && (int64_t)o.n < (int64_t)rows * nsm) rows = (rows + 1) / 2;
+    const int grid = (o.n + rows - 1) / rows;
+    if (dtype == PC_DT_F32) return launch_k(kv_store_kernel<S, float>, dim3(grid), dim3(256), 0, st, o, rows);
+    if (dtype == PC_DT_F16) return launch_k(kv_store_kernel<S, __half>, dim3(grid), dim3(256), 0, st, o, rows);
+    return launch_k(kv_store_kernel<S, __nv_bfloat16>, dim3(grid), dim3(256), 0, st, o, rows);
 }
 
 }  // namespace
 
 cudaError_t launch_kv_tables(const pc_kv_step &s, cudaStream_t st) {
-    return launch_k(kv_tables_kernel, dim3(1), dim3(TAB_THREADS), 0, st, s);
+    const cudaError_t e = launch_k(kv_tables_kernel, dim3(1), dim3(TAB_THREADS), 0, st, s);
+    if (e != cudaSuccess || s.n_tokens <= TAB_ROWS) return e;
+    return launch_k(kv_slots_kernel, dim3((s.n_tokens + 255) / 256), dim3(256), 0, st, s);
 }
 
 cudaError_t launch_kv_store(const pc_kv_pages &kv, const void *k, const int64_t *ks, const void *v, const int64_t *vs,
@@ -200,11 +279,9 @@ cudaError_t launch_kv_store(const pc_kv_pages &kv, const void *k, const int64_t 
     o.page = kv.page_size;
     o.KVH = kv.n_kv_heads;
     o.D = kv.head_dim;
-    const int64_t work = (int64_t)n * o.KVH * (o.D / 8);
-    const int grid = (int)std::min<int64_t>((work + 255) / 256, (int64_t)nsm * 8);
-    if (src_dtype == PC_DT_F32) return store_to<float>(o, kv.dtype, grid, st);
-    if (src_dtype == PC_DT_F16) return store_to<__half>(o, kv.dtype, grid, st);
-    return store_to<__nv_bfloat16>(o, kv.dtype, grid, st);
+    if (src_dtype == PC_DT_F32) return store_to<float>(o, kv.dtype, nsm, st);
+    if (src_dtype == PC_DT_F16) return store_to<__half>(o, kv.dtype, nsm, st);
+    return store_to<__nv_bfloat16>(o, kv.dtype, nsm, st);
 }
 
 }  // namespace pc

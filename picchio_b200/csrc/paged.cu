@@ -179,9 +179,8 @@ pc_status pc_kv_store(int device, const pc_kv_pages *kv, const void *k_dev, cons
         return fail(PC_ERR_FORMAT, "k and v need 16-byte aligned pointers and strides");
     OnDevice on(device);
     PC_CU(on.e);
-    int nsm = 148;
-    PC_CU(cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, device));
-    PC_CU(launch_kv_store(*kv, k_dev, k_stride, v_dev, v_stride, src_dtype, slot_dev, n, nsm, (cudaStream_t)stream));
+    constexpr int NSM = 148;  // only how small the blocks are cut hangs on it
+    PC_CU(launch_kv_store(*kv, k_dev, k_stride, v_dev, v_stride, src_dtype, slot_dev, n, NSM, (cudaStream_t)stream));
     return PC_OK;
 }
 

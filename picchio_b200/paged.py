@@ -19,7 +19,8 @@ DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 
 class _Pages(C.Structure):
-    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("ks0", C.c_int64), ("ks1", C.c_int64), ("ks2", C.c_int64),
+                ("vs0", C.c_int64), ("vs1", C.c_int64), ("vs2", C.c_int64),
                 ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int),
                 ("head_dim", C.c_int)]
 
@@ -32,7 +33,8 @@ class _Step(C.Structure):
 
 
 class _Call(C.Structure):
-    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64 * 2), ("out", C.c_void_p), ("out_stride", C.c_int64 * 2),
+    _fields_ = [("q", C.c_void_p), ("qs0", C.c_int64), ("qs1", C.c_int64), ("out", C.c_void_p), ("os0", C.c_int64),
+                ("os1", C.c_int64),
                 ("dtype", C.c_int), ("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
                 ("n_rows", C.c_int), ("n_requests", C.c_int), ("cu_new", C.c_void_p), ("sinks", C.c_void_p),
                 ("window", C.c_int), ("scale", C.c_float)]
@@ -50,6 +52,7 @@ class StepTables(NamedTuple):
 
 _L = None
 _dt = {}
+_Two = C.c_int64 * 2
 
 
 def _entry():
@@ -69,7 +72,11 @@ def _entry():
         for n in ("pc_kv_tables", "pc_kv_store", "pc_attn_create", "pc_attn_paged", "pc_attn_packed",
                   "pc_attn_check"):
             getattr(L, n).restype = C.c_int
-        _dt.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16})
+        _dt.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, "i32": torch.int32,
+                    "i64": torch.int64, "empty": torch.empty,
+                    # the current stream's handle without a Stream object (5 us less a call), where torch has it
+                    "stream": getattr(torch._C, "_cuda_getCurrentRawStream", None)
+                    or (lambda i: torch.cuda.current_stream(i).cuda_stream)})
         _L = L
     return _L
 
@@ -77,8 +84,7 @@ def _entry():
 def _stream(dev, stream):
     if stream is not None:
         return getattr(stream, "cuda_stream", stream)
-    import torch
-    return torch.cuda.current_stream(dev).cuda_stream
+    return _dt["stream"](dev.index)
 
 
 def _type(t, name):
@@ -88,34 +94,30 @@ def _type(t, name):
     return d
 
 
-def _ints(t, name, dev, n=None, dtype="int32"):
+def _ints(t, name, dev, n=None, dtype="i32"):
     """Pointer of a contiguous integer tensor on `dev` (of n elements, if given)."""
-    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or t.device != dev or (n is not None and t.numel() != n):
-        raise ValueError(f"{name}: a contiguous {dtype} tensor{'' if n is None else f' of {n} elements'} on {dev} expected")
+    if t.dtype != _dt[dtype] or not t.is_contiguous() or t.device != dev or (n is not None and t.numel() != n):
+        raise ValueError(f"{name}: a contiguous {_dt[dtype]} tensor{'' if n is None else f' of {n} elements'} on {dev} expected")
     return t.data_ptr()
 
 
 def _heads3(t, name, dev):
-    """A [rows, heads, head_dim] tensor with contiguous head_dim."""
-    if t.dim() != 3 or t.device != dev or (t.stride(2) != 1 and t.shape[2] != 1):
+    """(shape, strides) of a [rows, heads, head_dim] tensor with contiguous head_dim."""
+    shape, st = t.shape, t.stride()
+    if len(shape) != 3 or t.device != dev or (st[2] != 1 and shape[2] != 1):
         raise ValueError(f"{name}: a [rows, heads, head_dim] tensor on {dev} with contiguous head_dim expected")
-    return t
+    return shape, st
 
 
 def _pages(k_pages, v_pages) -> _Pages:
-    p = _Pages()
     shape = k_pages.shape
     ks, vs = k_pages.stride(), v_pages.stride()
     if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype or v_pages.device != k_pages.device \
             or not k_pages.is_cuda or ks[3] != 1 or vs[3] != 1:
         raise ValueError("k_pages, v_pages: two CUDA tensors [pages, page_size, kv_heads, head_dim] of one type with "
                          "contiguous head_dim expected")
-    p.k, p.v = k_pages.data_ptr(), v_pages.data_ptr()
-    p.k_stride[:] = ks[:3]
-    p.v_stride[:] = vs[:3]
-    p.dtype = _type(k_pages, "k_pages")
-    p.n_pages, p.page_size, p.n_kv_heads, p.head_dim = shape
-    return p
+    return _Pages(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                  _type(k_pages, "k_pages"), shape[0], shape[1], shape[2], shape[3])
 
 
 def kv_tables(kv_len, new_len, page_table, free_pages, n_free, *, page_size: int, n_tokens: int, stream=None) -> StepTables:
@@ -127,25 +129,22 @@ def kv_tables(kv_len, new_len, page_table, free_pages, n_free, *, page_size: int
     the next step's ``kv_len`` and ``n_free`` are returned.  ``n_tokens`` is
     the number of rows of the step's token tensors.
     """
-    import torch
     L = _entry()
     dev = kv_len.device
     B = kv_len.numel()
     if page_table.dim() != 2 or page_table.shape[0] != B or n_tokens < 0:
         raise ValueError("page_table: [requests, max_pages] expected, and n_tokens >= 0")
-    s = _Step()
-    s.n_requests, s.max_pages, s.page_size, s.n_tokens, s.free_cap = B, page_table.shape[1], page_size, n_tokens, free_pages.numel()
-    s.kv_len, s.new_len = _ints(kv_len, "kv_len", dev), _ints(new_len, "new_len", dev, B)
-    s.n_free = _ints(n_free, "n_free", dev, 1)
-    s.page_table, s.free_pages = _ints(page_table, "page_table", dev), _ints(free_pages, "free_pages", dev)
     # one allocation: cu_new, kv_end, served, n_free, positions
-    buf = torch.empty(3 * B + 2 + n_tokens, dtype=torch.int32, device=dev)
-    slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
-    out = StepTables(buf[B + 1:2 * B + 1], buf[:B + 1], buf[2 * B + 1:3 * B + 1], buf[3 * B + 1:3 * B + 2],
-                     buf[3 * B + 2:], slots)
+    empty = _dt["empty"]
+    buf = empty(3 * B + 2 + n_tokens, dtype=_dt["i32"], device=dev)
+    slots = empty(n_tokens, dtype=_dt["i64"], device=dev)
+    cu, end, served, left, pos = buf.split_with_sizes((B + 1, B, B, 1, n_tokens))
+    out = StepTables(end, cu, served, left, pos, slots)
     base = buf.data_ptr()
-    s.cu_new, s.kv_end, s.served = base, base + 4 * (B + 1), base + 4 * (2 * B + 1)
-    s.n_free_out, s.pos, s.slot = base + 4 * (3 * B + 1), base + 4 * (3 * B + 2), slots.data_ptr()
+    s = _Step(B, page_table.shape[1], page_size, n_tokens, free_pages.numel(), _ints(kv_len, "kv_len", dev),
+              _ints(new_len, "new_len", dev, B), _ints(n_free, "n_free", dev, 1),
+              _ints(page_table, "page_table", dev), _ints(free_pages, "free_pages", dev), base + 4 * (B + 1), base,
+              base + 4 * (2 * B + 1), base + 4 * (3 * B + 1), base + 4 * (3 * B + 2), slots.data_ptr())
     _check(L.pc_kv_tables(dev.index, C.byref(s), _stream(dev, stream)))
     return out
 
@@ -157,13 +156,12 @@ def kv_store(k_pages, v_pages, k, v, slots, stream=None) -> None:
     L = _entry()
     p = _pages(k_pages, v_pages)
     dev, n = k_pages.device, slots.numel()
-    _heads3(k, "k", dev)
-    _heads3(v, "v", dev)
-    if k.shape != v.shape or k.dtype != v.dtype or k.shape != (n, p.n_kv_heads, p.head_dim):
+    shape, ks = _heads3(k, "k", dev)
+    vshape, vs = _heads3(v, "v", dev)
+    if shape != vshape or k.dtype != v.dtype or shape != (n, p.n_kv_heads, p.head_dim):
         raise ValueError(f"k and v: two tensors [{n}, {p.n_kv_heads}, {p.head_dim}] of one type expected")
-    ks, vs = (C.c_int64 * 2)(*k.stride()[:2]), (C.c_int64 * 2)(*v.stride()[:2])
-    _check(L.pc_kv_store(dev.index, C.byref(p), k.data_ptr(), ks, v.data_ptr(), vs, _type(k, "k"),
-                         _ints(slots, "slots", dev, dtype="int64"), n, _stream(dev, stream)))
+    _check(L.pc_kv_store(dev.index, C.byref(p), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
+                         _type(k, "k"), _ints(slots, "slots", dev, dtype="i64"), n, _stream(dev, stream)))
 
 
 class Attention:
@@ -176,31 +174,26 @@ class Attention:
         self._h, self.device = h, device
 
     def _call(self, q, cu_new, sinks, window, scale, kv_heads, out):
-        import torch
-        if not q.is_cuda or q.device.index != self.device:
-            raise ValueError(f"q: a tensor on cuda:{self.device} expected")
         dev = q.device
-        _heads3(q, "q", dev)
-        T, H, D = q.shape
+        if dev.type != "cuda" or dev.index != self.device:
+            raise ValueError(f"q: a tensor on cuda:{self.device} expected")
+        shape, qs = _heads3(q, "q", dev)
+        T, H, D = shape
         if out is None:
-            out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out: a tensor like q expected")
-        _heads3(out, "out", dev)
-        c = _Call()
-        c.q, c.out = q.data_ptr(), out.data_ptr()
-        c.q_stride[:] = q.stride()[:2]
-        c.out_stride[:] = out.stride()[:2]
-        c.dtype, c.n_heads, c.n_kv_heads, c.head_dim, c.n_rows = _type(q, "q"), H, kv_heads, D, T
-        c.n_requests = cu_new.numel() - 1
-        c.cu_new = _ints(cu_new, "cu_new", dev)
+            out = _dt["empty"](shape, dtype=q.dtype, device=dev)
+            os = (H * D, D)
+        else:
+            oshape, os = _heads3(out, "out", dev)
+            if oshape != shape or out.dtype != q.dtype:
+                raise ValueError("out: a tensor like q expected")
+        sp = None
         if sinks is not None:
-            if sinks.dtype != torch.float32 or sinks.numel() != H or not sinks.is_contiguous() or sinks.device != dev:
+            if _dt.get(sinks.dtype) != DT_F32 or sinks.numel() != H or not sinks.is_contiguous() or sinks.device != dev:
                 raise ValueError(f"sinks: a contiguous float32 tensor of {H} elements on {dev} expected")
-            c.sinks = sinks.data_ptr()
-        c.window = int(window)
-        c.scale = D ** -0.5 if scale is None else scale
-        return c, out
+            sp = sinks.data_ptr()
+        return _Call(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], _type(q, "q"), H, kv_heads, D, T,
+                     cu_new.numel() - 1, _ints(cu_new, "cu_new", dev), sp, int(window),
+                     D ** -0.5 if scale is None else scale), out
 
     def paged(self, q, k_pages, v_pages, page_table, cu_new, kv_len, *, sinks=None, window: int = 0, scale=None,
               out=None, stream=None):
@@ -226,12 +219,12 @@ class Attention:
         rows ``cu_new[b] : cu_new[b + 1]`` of prompt b."""
         c, out = self._call(q, cu_new, sinks, window, scale, k.shape[1], out)
         dev = q.device
-        _heads3(k, "k", dev)
-        _heads3(v, "v", dev)
-        if k.shape != v.shape or k.dtype != q.dtype or v.dtype != q.dtype or k.shape[0] != c.n_rows or k.shape[2] != c.head_dim:
+        shape, ks = _heads3(k, "k", dev)
+        vshape, vs = _heads3(v, "v", dev)
+        if shape != vshape or k.dtype != q.dtype or v.dtype != q.dtype or shape[0] != c.n_rows or shape[2] != c.head_dim:
             raise ValueError("k and v: [rows, kv_heads, head_dim] of q's rows, head_dim and type expected")
-        ks, vs = (C.c_int64 * 2)(*k.stride()[:2]), (C.c_int64 * 2)(*v.stride()[:2])
-        _check(_L.pc_attn_packed(self._h, C.byref(c), k.data_ptr(), ks, v.data_ptr(), vs, _stream(dev, stream)))
+        _check(_L.pc_attn_packed(self._h, C.byref(c), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
+                                 _stream(dev, stream)))
         return out
 
     def check(self, stream=None):

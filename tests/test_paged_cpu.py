@@ -29,7 +29,9 @@ def test_bad_arguments_are_refused_without_a_device():
     assert L.pc_kv_store(0, C.byref(p), 16, two, 16, two, 0, 16, 1, None) == 1
     p.k = p.v = 4096
     p.n_pages, p.n_kv_heads, p.head_dim, p.page_size, p.dtype = 4, 2, 64, 16, 2
-    p.k_stride[:] = p.v_stride[:] = [16 * 2 * 64, 2 * 64, 64]
+    p.ks0 = p.vs0 = 16 * 2 * 64
+    p.ks1 = p.vs1 = 2 * 64
+    p.ks2 = p.vs2 = 64
     assert L.pc_kv_store(0, C.byref(p), 4096, two, 4096, two, 5, 4096, 1, None) == 3
     assert L.pc_kv_store(0, C.byref(p), 4098, two, 4096, two, 0, 4096, 1, None) == 3
     assert L.pc_kv_store(0, C.byref(p), 4096, two, 4096, two, 0, 4096, 0, None) == 0  # nothing to do
