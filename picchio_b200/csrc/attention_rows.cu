@@ -851,7 +851,9 @@ bool kv_tensor_map(const AttnOp &a, bool v, int dtype, int box, CUtensorMap &m) 
     const cuuint32_t boxes[4] = {64u, (cuuint32_t)box, 1u, 1u}, es[4] = {1u, 1u, 1u, 1u};
     return fn(&m, dtype == PC_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
               a.table ? 4 : 3, const_cast<void *>(v ? a.v : a.k), dims, strides, boxes, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              // what lies behind a head's row is another head's
+              a.D <= 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
