@@ -174,24 +174,6 @@ __device__ __forceinline__ void hide(uint32_t (&sv)[32], uint32_t seen) {
         if (!(seen >> y & 1u)) sv[y] = 0xFF800000u;
 }
 
-__device__ __forceinline__ uint64_t f2_pack_bits(uint32_t lo, uint32_t hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-    return d;
-}
-__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) { return f2_pack_bits(__float_as_uint(lo), __float_as_uint(hi)); }
-__device__ __forceinline__ float f2_lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float f2_hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 __device__ __forceinline__ uint64_t f2_ex2(uint64_t v) { return f2_pack(ex2(f2_lo(v)), ex2(f2_hi(v))); }
 // the largest of three, NaN if one of them is
 __device__ __forceinline__ float max3(float a, float b, float c) {

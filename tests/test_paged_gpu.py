@@ -273,6 +273,28 @@ def test_packed(dtype, lens, H, KH, D, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_heads_that_are_one(dtype):
+    """K and V expanded over heads (strides of zero): no tensor map has them."""
+    torch = _torch()
+    n, H, KH, D = 333, 6, 3, 64
+    g = gen(31)
+    q = torch.randn(n, H, D, generator=g, device="cuda").to(_dt(dtype))
+    k, v = (torch.randn(n, 1, D, generator=g, device="cuda").to(_dt(dtype)).expand(n, KH, D) for _ in range(2))
+    cu = torch.tensor([0, 100, n], dtype=torch.int32, device="cuda")
+    out = handle().packed(q, k, v, cu, window=50)
+    for a, b in ((0, 100), (100, n)):
+        want, bound = reference(q[a:b], k[a:b], v[a:b], 0, None, 50, D ** -0.5, dtype)
+        close(out[a:b], want, bound)
+    kp = torch.randn(8, 16, 1, D, generator=g, device="cuda").to(_dt(dtype)).expand(8, 16, KH, D)
+    table = torch.tensor([[3, 1, 7]], dtype=torch.int32, device="cuda")
+    for new in (1, 40):
+        cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+        out = handle().paged(q[:new], kp, kp, table, cu, torch.tensor([45], dtype=torch.int32, device="cuda"))
+        want, bound = reference(q[:new], gathered(kp, table, 0, 45), gathered(kp, table, 0, 45), 45 - new, None, 0, D ** -0.5, dtype)
+        close(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [64, 128])
 def test_unseen_keys_have_no_part(dtype, D):
     """NaN and infinities in K and V of positions that some rows do not see
