@@ -24,25 +24,20 @@
 // tile did not fit the instruction cache and spent more time waiting for
 // instructions than issuing them.
 //
-// The exponentials are the softmax's cost: at head size 64 a tile pair's
-// products take 1024 tensor cycles and its 32,768 exponentials 2048 cycles of
-// the special-function units (16 a cycle).  So in tiles without masked keys a
-// part of them runs on the FMA units instead: 2^x = 2^n 2^f, n the nearest
-// integer, 2^f on [-1/2, 1/2] by a polynomial of degree 3 (bf16 weights; its
-// relative error 7.5e-5 is 1/26 of the weight's rounding to bf16) or 4 (f16;
-// 2.7e-6, 1/90), fitted by reweighted least squares to the least maximal
-// relative error.
-//
-// The maximum that weights are taken against is moved only when a row's
-// maximum has grown by more than 2^8 (any reference within the exponent
-// range gives the same quotient), so O is hardly ever rescaled.
-//
+// Any reference within the exponent range gives the same quotient, so a row
+// keeps the one of its first tile, and later tiles are not searched for their
+// maximum first: the sum of 32 weights shows when one has grown past 2^14 (f16
+// weights, stored 2^7 up, end at 2^16), and then the tile is gone through the
+// careful way from there on: maximum, reference moved by a power of two, O and
+// what is written of the tile rescaled.
+
 // A key that a row does not see has weight 0, but 0 x NaN is NaN: in tiles
 // that some row does not see whole, V rows outside the item's keys (stale
 // pages) are zeroed and non-finite V elements of the others taken out before
 // the product; if there were any, the rows that see them get them added back
 // from global memory at the end of the item.
 #include <algorithm>
+#include <climits>
 
 #include "attention_half.cuh"
 #include "launch.cuh"
@@ -52,7 +47,8 @@ namespace pc {
 namespace {
 
 constexpr int RW_R = 256, RW_KT = 128, RW_OV = 384, RW_MINK = 256, RW_THREADS = 384;
-constexpr float RW_GROW = 8.0f;                     // log2 of the growth that moves the reference
+constexpr float RW_GROW = 8.0f;       // log2 of the growth that moves the reference in the careful way
+constexpr float RW_LIMIT = 16384.0f;  // what 32 weights of a row may sum up to before it is taken
 
 template <int HD>
 struct RowsCfg {
@@ -62,7 +58,7 @@ struct RowsCfg {
     static constexpr int QB = HD == 64 ? 2 : 1;   // Q buffers
     static constexpr int NB = HD == 64 ? 3 : 2;   // S / P buffers in TMEM, 128 columns each
     static constexpr int O0 = NB * 128;
-    static constexpr size_t SMEM = 1024 + (size_t)TILE * (2 * QB + 2 * STAGES) + 8 * 2048;  // 2 KB a row warp: output
+    static constexpr size_t SMEM = 1024 + (size_t)TILE * (2 * QB + 2 * STAGES);
     static constexpr int PART = RW_R * (HD + 2);
 };
 
@@ -182,39 +178,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-constexpr int RW_POLY = 6;  // of 16 pairs of exponentials, those on the FMA units
-
-// 2^x of both lanes: n = round(x) by adding 1.5 * 2^23, 2^(x - n) by a
-// polynomial (coefficients c[0] ...), n into the exponent.  x from -125 on (a
-// weight below 2^-125 of the largest counts as that) to 127.
-template <int DEG>
-__device__ __forceinline__ uint64_t f2_pow2(uint64_t x, const float (&c)[DEG + 1]) {
-    const uint64_t magic = f2_pack(12582912.0f, 12582912.0f);
-    x = f2_pack(fmaxf(f2_lo(x), -125.0f), fmaxf(f2_hi(x), -125.0f));
-    const uint64_t t = f2_add(x, magic), f = f2_sub(x, f2_sub(t, magic));
-    uint64_t p = f2_pack(c[DEG], c[DEG]);
-#pragma unroll
-    for (int i = DEG - 1; i >= 0; --i) p = f2_fma(p, f, f2_pack(c[i], c[i]));
-    return f2_pack_bits((uint32_t)p + ((uint32_t)t << 23), (uint32_t)(p >> 32) + ((uint32_t)(t >> 32) << 23));
-}
-
-// What part of the exponentials runs as f2_pow2 with, by the weights' type
-template <typename T>
-struct Pow2;
-template <>
-struct Pow2<__nv_bfloat16> {
-    static __device__ __forceinline__ uint64_t of(uint64_t x) {
-        return f2_pow2<3>(x, {0.9999280571937561f, 0.6932609677314758f, 0.2426111251115799f, 0.0551716685295105f});
-    }
-};
-template <>
-struct Pow2<__half> {
-    static __device__ __forceinline__ uint64_t of(uint64_t x) {
-        return f2_pow2<4>(x, {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f, 0.05591785907745361f,
-                              0.009570102207362652f});
-    }
-};
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(RW_THREADS, 1)
     attn_rows_kernel(const AttnOp a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -224,7 +187,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
     constexpr int NS = C::STAGES, QB = C::QB;
     extern __shared__ uint8_t rows_smem_raw[];
     uint8_t *smem = rows_smem_raw + (1024 - (smem_u32(rows_smem_raw) & 1023)) % 1024;
-    uint8_t *qs = smem, *ks = qs + 2 * C::QB * C::TILE, *vs = ks + NS * C::TILE, *os = vs + NS * C::TILE;
+    uint8_t *qs = smem, *ks = qs + 2 * C::QB * C::TILE, *vs = ks + NS * C::TILE;
     __shared__ PlanScratch<RW_THREADS> sc;
     __shared__ RowsBars bar;
     __shared__ uint32_t tmem_slot;
@@ -545,7 +508,6 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
         const int t = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, ot = tm + lanes + C::O0 + t * HD;
         const float c = __fmul_rn(a.scale, 1.4426950408889634f);
-        uint8_t *ow = os + warp * 2048;
         PlanWalk<RW_R, RW_KT> w(a, sc.share);
         int it = 0, item = 0;  // key tiles and items done
         uint32_t both_n = 0;
@@ -567,105 +529,125 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             const int f = g.r0 + t * 128 + r, tok = div_g(a, f);
             const int pos = f < g.r1 ? w.s.p0 + tok : -1;
             const float sink = a.sinks && f < g.r1 ? __fmul_rn(a.sinks[w.kvh * a.G + f - tok * a.G], 1.4426950408889634f) : 0.0f;
-            float m = -INFINITY, l = 0.0f;  // reference (of the scores as they are), sum
+            // positions of the warp's rows, lowest and highest
+            const int plo = __reduce_min_sync(0xffffffffu, pos < 0 && f >= g.r1 ? INT_MAX : pos),
+                      phi = __reduce_max_sync(0xffffffffu, pos);
+            float mr = f < g.r1 ? -INFINITY : 0.0f, l = 0.0f;  // reference in powers of two, sum
             for (int j = w.tl; j < w.th; ++j, ++it) {
                 const int n = 2 * it + t, b = n % C::NB;
                 const uint32_t st = tm + lanes + b * 128;
                 ok = wait_all(&bar.s_full[b], (n / C::NB) & 1);
                 if (!ok) break;
                 tc_fence_after();
-                const bool mk = masked(g, j);
-                const int hi = pos - (g.t0 + j) * RW_KT, lo = a.window > 0 ? hi - a.window : -1;  // sees lo < x <= hi
+                const int k0 = (g.t0 + j) * RW_KT, hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1;  // sees lo < x <= hi
+                // of the four groups of 32 keys, those that some row of the warp sees, and those that all see
+                const int x0 = a.window > 0 ? max((min(plo, phi) - a.window - k0 + 1) >> 5, 0) : 0;
+                const int x1 = phi < k0 ? -1 : min((phi - k0) >> 5, 3);
+                auto all_see = [&](int x) { return 32 * x + 31 <= plo - k0 && (a.window == 0 || 32 * x > phi - a.window - k0); };
                 uint32_t sv[32];
-                float mx;
-                if (!mk) {
-                    uint32_t sw[32];
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    tmem_ld32(st, sv);
-                    tmem_ld_wait32(sv);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {  // the next 32 columns come while these are compared
-                        uint32_t *cur = x & 1 ? sw : sv, *nxt = x & 1 ? sv : sw;
-                        if (x < 3) tmem_ld32(st + 32 * x + 32, nxt);
-#pragma unroll
-                        for (int y = 0; y < 16; ++y)
-                            top[y & 3] = max3(top[y & 3], __uint_as_float(cur[2 * y]), __uint_as_float(cur[2 * y + 1]));
-                        if (x < 3) tmem_ld_wait32(nxt);
-                    }
-                    mx = max3(max3(top[0], top[1], top[2]), top[3], -INFINITY);
-                } else {
-                    mx = -INFINITY;
-#pragma unroll 1
-                    for (int x = 0; x < 128; x += 32) {
-                        const uint32_t seen = seen_bits(lo - x, hi - x);
-                        if (!__any_sync(0xffffffffu, seen != 0)) continue;
-                        tmem_ld32(st + x, sv);
-                        tmem_ld_wait32(sv);
-                        hide(sv, seen);
-#pragma unroll
-                        for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
-                    }
-                }
-                // move the reference of rows whose maximum has grown
-                const bool first = m == -INFINITY;
-                const bool grow = !first && __fmul_rn(__fsub_rn(mx, m), c) > RW_GROW;
-                float corr = 1.0f;
-                if (grow) corr = ex2(__fmul_rn(__fsub_rn(m, mx), c));
-                if (first || grow || mx != mx) m = mx;
-                l = __fmul_rn(l, corr);
-                if (__any_sync(0xffffffffu, grow)) {
-                    ok = o_done();
-                    if (!ok) break;
-#pragma unroll 1
-                    for (int x = 0; x < HD; x += 16) {
-                        uint32_t ov[16];
-                        tmem_ld16(ot + x, ov);
-                        tmem_ld_wait16(ov);
-#pragma unroll
-                        for (int y = 0; y < 16; ++y) ov[y] = __float_as_uint(__fmul_rn(__uint_as_float(ov[y]), corr));
-                        tmem_st16(ot + x, ov);
-                    }
-                }
-                // weights 2^(s c - reference); an infinite or NaN reference makes all of them NaN
-                const float nmc = m == -INFINITY ? 0.0f : __fmaf_rn(m, 0.0f, __fsub_rn(E::BIAS, __fmul_rn(m, c)));
-                const uint64_t c2 = f2_pack(c, c), nmc2 = f2_pack(nmc, nmc);
                 uint64_t sum[2] = {0, 0};
-                tmem_ld32(st, sv);
+                const uint64_t c2 = f2_pack(c, c);
+                int xs = 0;  // the group from which on the careful way goes
+                bool grown = false;
+                if (all_see(0) && all_see(3) && __all_sync(0xffffffffu, mr != -INFINITY)) {
+                    // No look at the maximum first: the weights are taken against the reference as it is, and the
+                    // sum of a group tells whether one has grown too large for it (or is no number).
+                    const float nmc = __fsub_rn(E::BIAS, mr);
+                    const uint64_t nmc2 = f2_pack(nmc, nmc);
+                    tmem_ld32(st, sv);
 #pragma unroll 1
-                for (int x = 0; x < 4; ++x) {
-                    uint64_t v[16];
-                    uint32_t pk[16];
-                    tmem_ld_wait32(sv);
-                    bool some = true, full = true;
-                    if (mk) {
-                        const uint32_t seen = seen_bits(lo - 32 * x, hi - 32 * x);
-                        some = __any_sync(0xffffffffu, seen != 0);
-                        full = __all_sync(0xffffffffu, seen == ~0u);
-                        if (some && !full) hide(sv, seen);
-                    }
+                    for (; xs < 4; ++xs) {
+                        uint64_t v[16], part[2] = {0, 0};
+                        uint32_t pk[16];
+                        tmem_ld_wait32(sv);
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) v[y] = f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2);
-                    if (x < 3) tmem_ld32(st + 32 * x + 32, sv);
-                    if (full) {
-#pragma unroll
-                        for (int y = 0; y < 16; ++y) {
-                            // RW_POLY of 16 pairs on the FMA units, spread among the others
-                            const uint64_t p = (y * RW_POLY) % 16 < RW_POLY ? Pow2<T>::of(v[y]) : f2_ex2(v[y]);
-                            sum[y & 1] = f2_add(sum[y & 1], p);
-                            pk[y] = E::pack(f2_lo(p), f2_hi(p));
-                        }
-                    } else if (some) {  // an unseen key's weight is 0 and nothing else
+                        for (int y = 0; y < 16; ++y) v[y] = f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2);
+                        if (xs < 3) tmem_ld32(st + 32 * xs + 32, sv);
 #pragma unroll
                         for (int y = 0; y < 16; ++y) {
                             const uint64_t p = f2_ex2(v[y]);
-                            sum[y & 1] = f2_add(sum[y & 1], p);
+                            part[y & 1] = f2_add(part[y & 1], p);
                             pk[y] = E::pack(f2_lo(p), f2_hi(p));
                         }
-                    } else {
-#pragma unroll
-                        for (int y = 0; y < 16; ++y) pk[y] = 0;
+                        part[0] = f2_add(part[0], part[1]);
+                        if (__any_sync(0xffffffffu, !(__fadd_rn(f2_lo(part[0]), f2_hi(part[0])) <= RW_LIMIT))) {
+                            grown = true;
+                            break;
+                        }
+                        sum[xs & 1] = f2_add(sum[xs & 1], part[0]);
+                        tmem_st16(st + 16 * xs, pk);  // over columns read by now
                     }
-                    tmem_st16(st + 16 * x, pk);  // over columns read by now
+                    tmem_ld_wait32(sv);
+                }
+                if (xs < 4) {
+                    // the careful way, from group xs on: first tiles, tiles that some row does not see whole
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int x = max(x0, xs); x <= x1; ++x) {
+                        tmem_ld32(st + 32 * x, sv);
+                        tmem_ld_wait32(sv);
+                        if (!all_see(x)) hide(sv, seen_bits(lo - 32 * x, hi - 32 * x));
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
+                    }
+                    // move the reference of rows that have none, or whose maximum has grown
+                    const float top = __fmul_rn(mx, c), grow = ceilf(__fsub_rn(top, mr));
+                    float corr = 1.0f;
+                    if (mr == -INFINITY) {
+                        mr = top;
+                    } else if (grow > (grown ? 0.0f : RW_GROW)) {
+                        mr = __fadd_rn(mr, grow);
+                        corr = grow < 126.0f ? __int_as_float((127 - (int)grow) << 23) : 0.0f;
+                    }
+                    if (!(mx < INFINITY)) mr = NAN;  // an infinite or NaN score: so are the row's weights
+                    if (__any_sync(0xffffffffu, corr != 1.0f)) {
+                        ok = o_done();
+                        if (!ok) break;
+                        l = __fmul_rn(l, corr);
+                        sum[0] = f2_mul(sum[0], f2_pack(corr, corr));
+                        sum[1] = f2_mul(sum[1], f2_pack(corr, corr));
+#pragma unroll 1
+                        for (int x = 0; x < HD; x += 16) {
+                            uint32_t ov[16];
+                            tmem_ld16(ot + x, ov);
+                            tmem_ld_wait16(ov);
+#pragma unroll
+                            for (int y = 0; y < 16; ++y) ov[y] = __float_as_uint(__fmul_rn(__uint_as_float(ov[y]), corr));
+                            tmem_st16(ot + x, ov);
+                        }
+                        tmem_st_wait();
+#pragma unroll 1
+                        for (int x = 0; x < 16 * xs; x += 16) {  // weights of this tile that are written: exact, corr is a power of two
+                            uint32_t ov[16];
+                            tmem_ld16(st + x, ov);
+                            tmem_ld_wait16(ov);
+#pragma unroll
+                            for (int y = 0; y < 16; ++y)
+                                ov[y] = E::pack(__fmul_rn(E::up(ov[y] & 0xFFFFu), corr), __fmul_rn(E::up(ov[y] >> 16), corr));
+                            tmem_st16(st + x, ov);
+                        }
+                    }
+                    const float nmc = mr == -INFINITY ? 0.0f : __fsub_rn(E::BIAS, mr);
+                    const uint64_t nmc2 = f2_pack(nmc, nmc);
+#pragma unroll 1
+                    for (; xs < 4; ++xs) {
+                        uint32_t pk[16];
+                        if (xs >= x0 && xs <= x1) {
+                            tmem_ld32(st + 32 * xs, sv);
+                            tmem_ld_wait32(sv);
+                            if (!all_see(xs)) hide(sv, seen_bits(lo - 32 * xs, hi - 32 * xs));
+#pragma unroll
+                            for (int y = 0; y < 16; ++y) {
+                                const uint64_t p = f2_ex2(f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2));
+                                sum[y & 1] = f2_add(sum[y & 1], p);
+                                pk[y] = E::pack(f2_lo(p), f2_hi(p));
+                            }
+                        } else {
+#pragma unroll
+                            for (int y = 0; y < 16; ++y) pk[y] = 0;
+                        }
+                        tmem_st16(st + 16 * xs, pk);
+                    }
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -674,7 +656,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 l = __fadd_rn(l, __fadd_rn(f2_lo(both_sums), f2_hi(both_sums)));
             }
             if (!ok || !(ok = o_done())) break;
-            float mref = m == -INFINITY ? m : __fmul_rn(m, c);  // in powers of two
+            float mref = mr;
             // 32 columns of this block's O, with what masked tiles hold of non-finite V for the rows that see it
             auto own_o = [&](int x, float (&o)[32]) {
                 uint32_t ov[32];
@@ -735,9 +717,8 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 }
                 mref = mm;
             }
-            const bool none = mref == -INFINITY && l == 0.0f;  // no key seen
             const float inv = f < g.r1 ? row_factor<E>(mref, l, a.sinks != nullptr, sink) : 0.0f;
-            // through shared memory, so that four lanes write 64 bytes of a row
+            T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.s.q0 + tok) * a.os[0] + (int64_t)(w.kvh * a.G + f - tok * a.G) * a.os[1];
 #pragma unroll 1
             for (int x = 0; x < HD; x += 32) {
                 float o[32];
@@ -755,28 +736,16 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                         for (int d = 0; d < 32; ++d) o[d] = __fmaf_rn(__ldcg(p + (x + d) * RW_R), e, o[d]);
                     }
                 }
-                __syncwarp();
+                if (f < g.r1)
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
-                    uint32_t e[4];
+                    for (int ch = 0; ch < 4; ++ch)
+                        if (x + ch * 8 < a.D) {
+                            uint32_t e[4];
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        e[y] = none ? 0u : E::pack(__fmul_rn(o[ch * 8 + 2 * y], inv), __fmul_rn(o[ch * 8 + 2 * y + 1], inv));
-                    *reinterpret_cast<uint4 *>(ow + lane * 64 + ((ch ^ (lane >> 1 & 3)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
-                }
-                __syncwarp();
-                const int ch = lane & 3;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int rr = 8 * i + (lane >> 2), ff = g.r0 + t * 128 + (warp & 3) * 32 + rr;
-                    if (ff < g.r1 && x + ch * 8 < a.D) {
-                        const int ft = div_g(a, ff);
-                        T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.s.q0 + ft) * a.os[0] +
-                                 (int64_t)(w.kvh * a.G + ff - ft * a.G) * a.os[1] + x + ch * 8;
-                        *reinterpret_cast<uint4 *>(out) =
-                            *reinterpret_cast<const uint4 *>(ow + rr * 64 + ((ch ^ (rr >> 1 & 3)) << 4));
-                    }
-                }
+                            for (int y = 0; y < 4; ++y)  // a row without keys: 0 x 0
+                                e[y] = E::pack(__fmul_rn(o[ch * 8 + 2 * y], inv), __fmul_rn(o[ch * 8 + 2 * y + 1], inv));
+                            *reinterpret_cast<uint4 *>(out + x + ch * 8) = make_uint4(e[0], e[1], e[2], e[3]);
+                        }
             }
             tc_fence_before();
         }
