@@ -31,7 +31,7 @@ namespace pc {
 
 namespace {
 
-constexpr int FW_WARPS = 4, FW_THREADS = FW_WARPS * 32, FW_OV = 128, FW_MINK = 128;
+constexpr int FW_WARPS = 4, FW_THREADS = FW_WARPS * 32, FW_OV = 256, FW_MINK = 128;
 constexpr int FW_PER_SM = 2, FW_AHEAD = 1;  // blocks an SM; stages a warp
 
 template <int HD>

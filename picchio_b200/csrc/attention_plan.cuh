@@ -68,14 +68,21 @@ __device__ __forceinline__ ItemGeo item_geo(const AttnOp &a, const SeqGeo &s, in
     return g;
 }
 
+// a / b of numbers that are not negative: the 64-bit division is a routine of
+// its own, worth going round in the short calls, where the numbers are small
+__device__ __forceinline__ int64_t div_len(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
+}
+
 // Length of the first i items of a request and one KV head, in keys x group.
 template <int R, int KT, int OV>
 __device__ __forceinline__ int64_t items_len(const AttnOp &a, const SeqGeo &s, int i) {
     const int64_t A = (int64_t)s.p0 * a.G;
-    int64_t lo = A < 0 ? min((int64_t)i, -A / R) : 0;  // items without keys
+    int64_t lo = A < 0 ? min((int64_t)i, div_len(-A, R)) : 0;  // items without keys
     int64_t hi = i;                                     // from here on the window's length
     const int64_t W = (int64_t)a.window * a.G + R;
-    if (a.window > 0) hi = max(lo, min((int64_t)i, A >= W ? (int64_t)0 : (W - A) / R));
+    if (a.window > 0) hi = max(lo, min((int64_t)i, A >= W ? (int64_t)0 : div_len(W - A, R)));
     return (int64_t)i * OV * a.G + (hi - lo) * A + R * (hi * (hi + 1) - lo * (lo + 1)) / 2 + (i - hi) * W;
 }
 
@@ -101,14 +108,14 @@ struct PlanScratch {
     PlanShare share;
 };
 
-__device__ __forceinline__ int64_t share_start(int64_t total, int n, int k) { return total * k / n; }
+__device__ __forceinline__ int64_t share_start(int64_t total, int n, int k) { return div_len(total * k, n); }
 
 template <int R, int KT, int OV>
 __device__ __forceinline__ void plan_point(const AttnOp &a, int b, int64_t base, int64_t x, PlanPoint &p) {
     const SeqGeo s = seq_geo<R>(a, b);
     const int64_t per = items_len<R, KT, OV>(a, s, s.n_items);
     p.b = b;
-    p.kvh = (int)((x - base) / per);
+    p.kvh = (int)div_len(x - base, per);
     const int64_t r = (x - base) - p.kvh * per;
     int lo = 0, hi = s.n_items;  // items_len(lo) <= r < items_len(hi)
     while (hi - lo > 1) {
@@ -121,7 +128,7 @@ __device__ __forceinline__ void plan_point(const AttnOp &a, int b, int64_t base,
     p.len = items_len<R, KT, OV>(a, s, lo + 1) - c0;
     p.len0 = base + p.kvh * per + c0;
     const ItemGeo g = item_geo<R, KT>(a, s, lo);
-    p.tile = (int)((r - c0) * g.nt / p.len);
+    p.tile = (int)div_len((r - c0) * g.nt, p.len);
 }
 
 // The share of thread block `cta` of `ctas`; every thread of the block calls
@@ -147,15 +154,19 @@ __device__ void plan_share(const AttnOp &a, int cta, int ctas, PlanScratch<THREA
     // no share is shorter than an item's longest tile, so no share of an item
     // it touches is empty
     int64_t least = (int64_t)a.G * (max(KT, MINK) + OV + 1) + R + 1;
-    const int n = (int)max((int64_t)1, min((int64_t)ctas, total / least));
+    const int n = (int)max((int64_t)1, min((int64_t)ctas, div_len(total, least)));
     if (cta >= n || total == 0) {
         if (tid == 0) sc.share.n = 0;
         __syncthreads();
         return;
     }
     const int64_t x0 = share_start(total, n, cta), x1 = share_start(total, n, cta + 1);
+    if (a.B == 1 && tid < 2) {
+        sc.b[tid] = (tid ? x1 : x0) < total ? 0 : 1;
+        sc.base[tid] = 0;
+    }
     int64_t carry = 0;
-    for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+    for (int b0 = 0; b0 < (a.B == 1 ? 0 : a.B); b0 += THREADS) {
         const int b = b0 + tid;
         if (a.B > THREADS) {
             mine = 0;
@@ -262,9 +273,9 @@ __device__ __forceinline__ CutItem cut_item(const PlanWalk<R, KT> &w) {
     const int64_t total = w.sh.total;
     const int n = w.sh.n;
     CutItem c;
-    c.k0 = (int)(((p.len0 + 1) * n - 1) / total);
-    c.k1 = (int)(((p.len0 + p.len) * n - 1) / total);
-    if (c.k0 < c.k1 && (share_start(total, n, c.k0 + 1) - p.len0) * w.g.nt / p.len == 0) ++c.k0;
+    c.k0 = (int)div_len((p.len0 + 1) * n - 1, total);
+    c.k1 = (int)div_len((p.len0 + p.len) * n - 1, total);
+    if (c.k0 < c.k1 && (share_start(total, n, c.k0 + 1) - p.len0) * w.g.nt < p.len) ++c.k0;
     return c;
 }
 

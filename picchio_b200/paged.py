@@ -51,12 +51,15 @@ class StepTables(NamedTuple):
 
 
 _L = None
-_dt = {}
+_dt = {}           # torch dtype -> PC_DT_*
+_i32 = _i64 = None  # torch.int32, torch.int64
+_raw_stream = None  # device index -> handle of torch's current stream
 _Two = C.c_int64 * 2
+_byref = C.byref
 
 
 def _entry():
-    global _L
+    global _L, _i32, _i64, _raw_stream
     if _L is None:
         import torch
         L = lib()
@@ -72,19 +75,18 @@ def _entry():
         for n in ("pc_kv_tables", "pc_kv_store", "pc_attn_create", "pc_attn_paged", "pc_attn_packed",
                   "pc_attn_check"):
             getattr(L, n).restype = C.c_int
-        _dt.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, "i32": torch.int32,
-                    "i64": torch.int64, "empty": torch.empty,
-                    # the current stream's handle without a Stream object (5 us less a call), where torch has it
-                    "stream": getattr(torch._C, "_cuda_getCurrentRawStream", None)
-                    or (lambda i: torch.cuda.current_stream(i).cuda_stream)})
+        _dt.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16})
+        _i32, _i64 = torch.int32, torch.int64
+        # the current stream's handle without a Stream object (5 us less a call), where torch has it
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda i: torch.cuda.current_stream(i).cuda_stream)
         _L = L
     return _L
 
 
 def _stream(dev, stream):
-    if stream is not None:
-        return getattr(stream, "cuda_stream", stream)
-    return _dt["stream"](dev.index)
+    """The stream of a call on device `dev`: torch's current one unless given."""
+    return _raw_stream(dev) if stream is None else getattr(stream, "cuda_stream", stream)
 
 
 def _type(t, name):
@@ -94,28 +96,28 @@ def _type(t, name):
     return d
 
 
-def _ints(t, name, dev, n=None, dtype="i32"):
-    """Pointer of a contiguous integer tensor on `dev` (of n elements, if given)."""
-    if t.dtype != _dt[dtype] or not t.is_contiguous() or t.device != dev or (n is not None and t.numel() != n):
-        raise ValueError(f"{name}: a contiguous {_dt[dtype]} tensor{'' if n is None else f' of {n} elements'} on {dev} expected")
+def _ints(t, name, dev, n, dtype):
+    """Pointer of a contiguous integer tensor of n elements on device `dev`."""
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor of {n} elements on cuda:{dev} expected")
     return t.data_ptr()
 
 
 def _heads3(t, name, dev):
     """(shape, strides) of a [rows, heads, head_dim] tensor with contiguous head_dim."""
     shape, st = t.shape, t.stride()
-    if len(shape) != 3 or t.device != dev or (st[2] != 1 and shape[2] != 1):
-        raise ValueError(f"{name}: a [rows, heads, head_dim] tensor on {dev} with contiguous head_dim expected")
+    if len(shape) != 3 or t.get_device() != dev or (st[2] != 1 and shape[2] != 1):
+        raise ValueError(f"{name}: a [rows, heads, head_dim] tensor on cuda:{dev} with contiguous head_dim expected")
     return shape, st
 
 
-def _pages(k_pages, v_pages) -> _Pages:
+def _pages(k_pages, v_pages, dev) -> _Pages:
     shape = k_pages.shape
     ks, vs = k_pages.stride(), v_pages.stride()
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype or v_pages.device != k_pages.device \
-            or not k_pages.is_cuda or ks[3] != 1 or vs[3] != 1:
-        raise ValueError("k_pages, v_pages: two CUDA tensors [pages, page_size, kv_heads, head_dim] of one type with "
-                         "contiguous head_dim expected")
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype or k_pages.get_device() != dev \
+            or v_pages.get_device() != dev or ks[3] != 1 or vs[3] != 1:
+        raise ValueError(f"k_pages, v_pages: two tensors [pages, page_size, kv_heads, head_dim] of one type on cuda:{dev} "
+                         "with contiguous head_dim expected")
     return _Pages(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
                   _type(k_pages, "k_pages"), shape[0], shape[1], shape[2], shape[3])
 
@@ -130,23 +132,24 @@ def kv_tables(kv_len, new_len, page_table, free_pages, n_free, *, page_size: int
     the number of rows of the step's token tensors.
     """
     L = _entry()
-    dev = kv_len.device
-    B = kv_len.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != B or n_tokens < 0:
-        raise ValueError("page_table: [requests, max_pages] expected, and n_tokens >= 0")
+    dev, B, width = kv_len.get_device(), kv_len.numel(), page_table.shape[-1]
+    if dev < 0 or page_table.shape != (B, width) or n_tokens < 0:
+        raise ValueError("kv_len on a CUDA device, page_table [requests, max_pages] and n_tokens >= 0 expected")
+    cap = free_pages.numel()
+    ptrs = (_ints(kv_len, "kv_len", dev, B, _i32), _ints(new_len, "new_len", dev, B, _i32),
+            _ints(n_free, "n_free", dev, 1, _i32), _ints(page_table, "page_table", dev, B * width, _i32),
+            _ints(free_pages, "free_pages", dev, cap, _i32))
     # one allocation: cu_new, kv_end, served, n_free, positions
-    empty = _dt["empty"]
-    buf = empty(3 * B + 2 + n_tokens, dtype=_dt["i32"], device=dev)
-    slots = empty(n_tokens, dtype=_dt["i64"], device=dev)
-    cu, end, served, left, pos = buf.split_with_sizes((B + 1, B, B, 1, n_tokens))
-    out = StepTables(end, cu, served, left, pos, slots)
+    buf = kv_len.new_empty(3 * B + 2 + n_tokens)
+    slots = kv_len.new_empty(n_tokens, dtype=_i64)
     base = buf.data_ptr()
-    s = _Step(B, page_table.shape[1], page_size, n_tokens, free_pages.numel(), _ints(kv_len, "kv_len", dev),
-              _ints(new_len, "new_len", dev, B), _ints(n_free, "n_free", dev, 1),
-              _ints(page_table, "page_table", dev), _ints(free_pages, "free_pages", dev), base + 4 * (B + 1), base,
-              base + 4 * (2 * B + 1), base + 4 * (3 * B + 1), base + 4 * (3 * B + 2), slots.data_ptr())
-    _check(L.pc_kv_tables(dev.index, C.byref(s), _stream(dev, stream)))
-    return out
+    end = base + 4 * (B + 1)
+    served = end + 4 * B
+    s = _Step(B, width, page_size, n_tokens, cap, *ptrs, end, base, served, served + 4 * B, served + 4 * B + 4,
+              slots.data_ptr())
+    _check(L.pc_kv_tables(dev, _byref(s), _stream(dev, stream)))
+    cu, end, served, left, pos = buf.split_with_sizes((B + 1, B, B, 1, n_tokens))
+    return StepTables(end, cu, served, left, pos, slots)
 
 
 def kv_store(k_pages, v_pages, k, v, slots, stream=None) -> None:
@@ -154,14 +157,16 @@ def kv_store(k_pages, v_pages, k, v, slots, stream=None) -> None:
     cache [pages, page_size, kv_heads, head_dim] (pc_kv_store), rounded to its
     type; rows with a slot outside the cache (-1) are skipped."""
     L = _entry()
-    p = _pages(k_pages, v_pages)
-    dev, n = k_pages.device, slots.numel()
+    dev, n = k.get_device(), slots.numel()
+    if dev < 0:
+        raise ValueError("k: a CUDA tensor expected")
+    p = _pages(k_pages, v_pages, dev)
     shape, ks = _heads3(k, "k", dev)
     vshape, vs = _heads3(v, "v", dev)
-    if shape != vshape or k.dtype != v.dtype or shape != (n, p.n_kv_heads, p.head_dim):
+    if shape != vshape or k.dtype is not v.dtype or shape != (n, p.n_kv_heads, p.head_dim):
         raise ValueError(f"k and v: two tensors [{n}, {p.n_kv_heads}, {p.head_dim}] of one type expected")
-    _check(L.pc_kv_store(dev.index, C.byref(p), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
-                         _type(k, "k"), _ints(slots, "slots", dev, dtype="i64"), n, _stream(dev, stream)))
+    _check(L.pc_kv_store(dev, _byref(p), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
+                         _type(k, "k"), _ints(slots, "slots", dev, n, _i64), n, _stream(dev, stream)))
 
 
 class Attention:
@@ -174,26 +179,24 @@ class Attention:
         self._h, self.device = h, device
 
     def _call(self, q, cu_new, sinks, window, scale, kv_heads, out):
-        dev = q.device
-        if dev.type != "cuda" or dev.index != self.device:
-            raise ValueError(f"q: a tensor on cuda:{self.device} expected")
+        dev = self.device
         shape, qs = _heads3(q, "q", dev)
         T, H, D = shape
         if out is None:
-            out = _dt["empty"](shape, dtype=q.dtype, device=dev)
+            out = q.new_empty(shape)
             os = (H * D, D)
         else:
             oshape, os = _heads3(out, "out", dev)
-            if oshape != shape or out.dtype != q.dtype:
+            if oshape != shape or out.dtype is not q.dtype:
                 raise ValueError("out: a tensor like q expected")
         sp = None
         if sinks is not None:
-            if _dt.get(sinks.dtype) != DT_F32 or sinks.numel() != H or not sinks.is_contiguous() or sinks.device != dev:
-                raise ValueError(f"sinks: a contiguous float32 tensor of {H} elements on {dev} expected")
+            if _dt.get(sinks.dtype) != DT_F32 or sinks.numel() != H or sinks.get_device() != dev or not sinks.is_contiguous():
+                raise ValueError(f"sinks: a contiguous float32 tensor of {H} elements on cuda:{dev} expected")
             sp = sinks.data_ptr()
-        return _Call(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], _type(q, "q"), H, kv_heads, D, T,
-                     cu_new.numel() - 1, _ints(cu_new, "cu_new", dev), sp, int(window),
-                     D ** -0.5 if scale is None else scale), out
+        n = cu_new.numel()
+        return _Call(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], _type(q, "q"), H, kv_heads, D, T, n - 1,
+                     _ints(cu_new, "cu_new", dev, n, _i32), sp, int(window), D ** -0.5 if scale is None else scale), out
 
     def paged(self, q, k_pages, v_pages, page_table, cu_new, kv_len, *, sinks=None, window: int = 0, scale=None,
               out=None, stream=None):
@@ -204,34 +207,34 @@ class Attention:
         head_dim]; ``page_table`` [B, max_pages], ``cu_new`` [B + 1],
         ``kv_len`` [B] int32: positions in the cache, the new rows' included.
         """
-        p = _pages(k_pages, v_pages)
+        dev = self.device
+        p = _pages(k_pages, v_pages, dev)
         c, out = self._call(q, cu_new, sinks, window, scale, p.n_kv_heads, out)
-        dev = q.device
-        if page_table.dim() != 2 or page_table.shape[0] != c.n_requests or k_pages.device != dev:
-            raise ValueError("page_table: [requests, max_pages] expected, on one device with q and the pages")
-        _check(_L.pc_attn_paged(self._h, C.byref(c), C.byref(p), _ints(page_table, "page_table", dev),
-                                page_table.shape[1], _ints(kv_len, "kv_len", dev, c.n_requests), _stream(dev, stream)))
+        B, width = c.n_requests, page_table.shape[-1]
+        if page_table.shape != (B, width):
+            raise ValueError(f"page_table: [{B}, max_pages] expected")
+        _check(_L.pc_attn_paged(self._h, _byref(c), _byref(p), _ints(page_table, "page_table", dev, B * width, _i32), width,
+                                _ints(kv_len, "kv_len", dev, B, _i32), _stream(dev, stream)))
         return out
 
     def packed(self, q, k, v, cu_new, *, sinks=None, window: int = 0, scale=None, out=None, stream=None):
         """Attention over whole prompts packed into one tensor (pc_attn_packed):
         ``q`` [rows, heads, head_dim], ``k``, ``v`` [rows, kv_heads, head_dim],
         rows ``cu_new[b] : cu_new[b + 1]`` of prompt b."""
-        c, out = self._call(q, cu_new, sinks, window, scale, k.shape[1], out)
-        dev = q.device
+        dev = self.device
         shape, ks = _heads3(k, "k", dev)
         vshape, vs = _heads3(v, "v", dev)
-        if shape != vshape or k.dtype != q.dtype or v.dtype != q.dtype or shape[0] != c.n_rows or shape[2] != c.head_dim:
+        c, out = self._call(q, cu_new, sinks, window, scale, shape[1], out)
+        if shape != vshape or k.dtype is not q.dtype or v.dtype is not q.dtype or shape[0] != c.n_rows or shape[2] != c.head_dim:
             raise ValueError("k and v: [rows, kv_heads, head_dim] of q's rows, head_dim and type expected")
-        _check(_L.pc_attn_packed(self._h, C.byref(c), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
+        _check(_L.pc_attn_packed(self._h, _byref(c), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
                                  _stream(dev, stream)))
         return out
 
     def check(self, stream=None):
         """pc_attn_check: waits for the stream and raises if an earlier call
         on this handle reported a device-side failure."""
-        import torch
-        _check(_L.pc_attn_check(self._h, _stream(torch.device("cuda", self.device), stream)))
+        _check(_L.pc_attn_check(self._h, _stream(self.device, stream)))
 
     def close(self):
         if getattr(self, "_h", None):
