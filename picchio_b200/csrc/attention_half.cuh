@@ -44,8 +44,9 @@ __device__ __forceinline__ bool mbar_sleep_wait(uint64_t *bar, uint32_t parity) 
 
 // A bounded wait of one of a block's threads: false once it, or any other
 // wait of the block, gave up (*dead, in shared memory); *err tells the host.
-__device__ __forceinline__ bool bounded_wait(uint64_t *bar, uint32_t parity, volatile int *dead, int *err) {
-    if (mbar_sleep_wait(bar, parity)) return true;
+// What comes after the first try is a function of its own: inlined at every
+// wait it filled the instruction cache.
+static __device__ __noinline__ bool bounded_wait_on(uint64_t *bar, uint32_t parity, volatile int *dead, int *err) {
     const long long t0 = clock64();
     while (!mbar_sleep_wait(bar, parity)) {
         if (*dead) return false;
@@ -56,6 +57,9 @@ __device__ __forceinline__ bool bounded_wait(uint64_t *bar, uint32_t parity, vol
         }
     }
     return true;
+}
+__device__ __forceinline__ bool bounded_wait(uint64_t *bar, uint32_t parity, volatile int *dead, int *err) {
+    return mbar_sleep_wait(bar, parity) || bounded_wait_on(bar, parity, dead, err);
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -46,7 +46,7 @@ namespace pc {
 
 namespace {
 
-constexpr int RW_R = 256, RW_KT = 128, RW_OV = 384, RW_MINK = 256, RW_THREADS = 384;
+constexpr int RW_R = 256, RW_KT = 128, RW_OV = 256, RW_MINK = 256, RW_THREADS = 384;
 constexpr float RW_GROW = 8.0f;       // log2 of the growth that moves the reference in the careful way
 constexpr float RW_LIMIT = 16384.0f;  // what 32 weights of a row may sum up to before it is taken
 
@@ -66,9 +66,21 @@ struct KeySteps {
     int lo, hi;
 };
 
+// An item of the block's share as all roles read it: warp 8 walks the share
+// (attention_plan.cuh) and leaves one after another, an item ahead of its
+// tiles.  (With the walk in every role its 64-bit arithmetic stood in each
+// one's way at every item, and five times in the instruction cache.)
+struct ItemDesc {
+    ItemGeo g;
+    int b, kvh, q0, p0;  // request, KV head, its first row, that row's position
+    int tl, th;          // this block's tiles; none: the share is done
+    int k0, k1;          // blocks that share the item; k0 < 0: it is whole
+};
+constexpr int RW_ITEMS = 4;  // descriptors in the ring
+
 struct RowsBars {
     uint64_t q_full[4], q_free[4], s_full[3], p_full[3], o_full[4];
-    uint64_t k_full[3], k_free[3], v_full[3], v_free[3], v_fixed[3], both, drain[2];
+    uint64_t k_full[3], k_free[3], v_full[3], v_free[3], v_fixed[3], d_full[RW_ITEMS], d_free[RW_ITEMS], both, drain[2];
 };
 
 __device__ __forceinline__ void cp_async16_fill(uint32_t dst, const void *src, int bytes) {
@@ -178,9 +190,130 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// A tile of keys (the block's tile t of an item) that some row of the item
+// does not see whole
+__device__ __forceinline__ bool rows_masked(const ItemGeo &g, int t, int window) {
+    const int k0 = (g.t0 + t) * RW_KT;
+    return k0 + RW_KT - 1 > g.pmin || (window > 0 && k0 < g.pmax - window + 1);
+}
+
+// What an item hardly ever or seldom needs is in functions of their own: the
+// row warps' loops share the instruction cache with all that is inlined (16
+// prompts to 2k took 7 % less with the waits' second half out alone).
+
+// Adds what masked tiles hold of non-finite V to the O of a row that sees it.
+template <typename T, int HD>
+__device__ __noinline__ void add_odd(const AttnOp &a, const ItemDesc w, int pos, uint32_t ot) {
+    const ItemGeo &g = w.g;
+    const T *vb = reinterpret_cast<const T *>(a.v) + (int64_t)w.kvh * a.vs[2];
+#pragma unroll 1
+    for (int x = 0; x < HD; x += 16) {
+        uint32_t o[16];
+        tmem_ld16(ot + x, o);
+        tmem_ld_wait16(o);
+        for (int key = (g.t0 + w.tl) * RW_KT; key < (g.t0 + w.th) * RW_KT; ++key) {
+            if (key < g.kb || key >= g.ke || key > pos || (a.window > 0 && key <= pos - a.window) ||
+                !rows_masked(g, key / RW_KT - g.t0, a.window))
+                continue;
+            const T *vp = vb + (int64_t)(w.q0 + key) * a.vs[1];
+            if (a.table) {
+                const int page = a.table[(int64_t)w.b * a.max_pages + key / a.page_size];
+                if (page < 0 || page >= a.n_pages) continue;
+                vp = vb + page * a.vs[0] + (int64_t)(key % a.page_size) * a.vs[1];
+            }
+#pragma unroll
+            for (int d = 0; d < 16; ++d) {
+                const float v = x + d < a.D ? Half16<T>::up(reinterpret_cast<const unsigned short *>(vp)[x + d]) : 0.0f;
+                if (!isfinite(v)) o[d] = __float_as_uint(__fadd_rn(__uint_as_float(o[d]), v));
+            }
+        }
+        __syncwarp();
+        tmem_st16(ot + x, o);
+    }
+    tmem_st_wait();
+}
+
+// A row's O, reference and sum to the workspace (`mine`: its place in the block's record).
+template <int HD>
+__device__ __noinline__ void leave_part(float *mine, uint32_t ot, float m, float l) {
+#pragma unroll 1
+    for (int x = 0; x < HD; x += 16) {
+        uint32_t o[16];
+        tmem_ld16(ot + x, o);
+        tmem_ld_wait16(o);
+#pragma unroll
+        for (int d = 0; d < 16; ++d) __stcg(mine + (x + d) * RW_R, __uint_as_float(o[d]));
+    }
+    __stcg(mine + HD * RW_R, m);
+    __stcg(mine + (HD + 1) * RW_R, l);
+}
+
+// The parts of blocks k0 .. k1 in block order: O into TMEM, (reference, sum).
+template <int HD>
+__device__ __noinline__ float2 join_parts(const float *part, int k0, int k1, uint32_t ot) {
+    auto of = [&](int k) { return part + ((int64_t)k * 2 + (k == k0)) * RowsCfg<HD>::PART; };
+    float mm = -INFINITY, l = 0.0f;
+#pragma unroll 4
+    for (int k = k0; k <= k1; ++k) mm = fmaxf(mm, __ldcg(of(k) + HD * RW_R));
+    const float ms = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll 4
+    for (int k = k0; k <= k1; ++k)
+        l = __fmaf_rn(__ldcg(of(k) + (HD + 1) * RW_R), ex2(__fsub_rn(__ldcg(of(k) + HD * RW_R), ms)), l);
+#pragma unroll 1
+    for (int x = 0; x < HD; x += 16) {
+        float o[16];
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[d] = 0.0f;
+#pragma unroll 2
+        for (int k = k0; k <= k1; ++k) {
+            const float *p = of(k);
+            const float e = ex2(__fsub_rn(__ldcg(p + HD * RW_R), ms));
+#pragma unroll
+            for (int d = 0; d < 16; ++d) o[d] = __fmaf_rn(__ldcg(p + (x + d) * RW_R), e, o[d]);
+        }
+        uint32_t ov[16];
+#pragma unroll
+        for (int d = 0; d < 16; ++d) ov[d] = __float_as_uint(o[d]);
+        __syncwarp();
+        tmem_st16(ot + x, ov);
+    }
+    tmem_st_wait();
+    return make_float2(mm, l);
+}
+
+// A row's O (`cols` columns) times corr
+static __device__ __noinline__ void scale_o(uint32_t ot, int cols, float corr) {
+#pragma unroll 1
+    for (int x = 0; x < cols; x += 16) {
+        uint32_t ov[16];
+        tmem_ld16(ot + x, ov);
+        tmem_ld_wait16(ov);
+#pragma unroll
+        for (int y = 0; y < 16; ++y) ov[y] = __float_as_uint(__fmul_rn(__uint_as_float(ov[y]), corr));
+        tmem_st16(ot + x, ov);
+    }
+    tmem_st_wait();
+}
+// Written weights (`cols` columns of two) times corr: exact, it is a power of two
+template <typename T>
+__device__ __noinline__ void scale_p(uint32_t st, int cols, float corr) {
+    using E = Half16<T>;
+#pragma unroll 1
+    for (int x = 0; x < cols; x += 16) {
+        uint32_t ov[16];
+        tmem_ld16(st + x, ov);
+        tmem_ld_wait16(ov);
+#pragma unroll
+        for (int y = 0; y < 16; ++y)
+            ov[y] = E::pack(__fmul_rn(E::up(ov[y] & 0xFFFFu), corr), __fmul_rn(E::up(ov[y] >> 16), corr));
+        tmem_st16(st + x, ov);
+    }
+    tmem_st_wait();
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(RW_THREADS, 1)
-    attn_rows_kernel(const AttnOp a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+    attn_rows_kernel(const __grid_constant__ AttnOp a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      const __grid_constant__ CUtensorMap qmap, const int box, const bool qtma) {
     using C = RowsCfg<HD>;
     using E = Half16<T>;
@@ -190,6 +323,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
     uint8_t *qs = smem, *ks = qs + 2 * C::QB * C::TILE, *vs = ks + NS * C::TILE;
     __shared__ PlanScratch<RW_THREADS> sc;
     __shared__ RowsBars bar;
+    __shared__ ItemDesc items[RW_ITEMS];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     __shared__ int lastf;
@@ -213,6 +347,10 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             mbar_init(&bar.v_free[s], 1);
             mbar_init(&bar.v_fixed[s], 32);
         }
+        for (int i = 0; i < RW_ITEMS; ++i) {
+            mbar_init(&bar.d_full[i], 1);
+            mbar_init(&bar.d_free[i], 11);  // the warps that read it
+        }
         mbar_init(&bar.both, 256);
         mbar_init(&bar.drain[0], 1);
         mbar_init(&bar.drain[1], 1);
@@ -234,6 +372,14 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
 
     auto wait = [&](uint64_t *b, uint32_t parity) -> bool { return bounded_wait(b, parity, &dead, a.err); };
     auto wait_all = [&](uint64_t *b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    // Item `i` of the share; false if the share is done (or a wait gave up: ok).
+    auto take = [&](int i, ItemDesc &d, bool &ok) -> bool {
+        if (!(ok = wait_all(&bar.d_full[i % RW_ITEMS], (i / RW_ITEMS) & 1))) return false;
+        d = items[i % RW_ITEMS];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.d_free[i % RW_ITEMS]);
+        return d.th > d.tl;
+    };
     // the steps of 16 keys of a tile that hold keys of the item (one at least)
     auto key_steps = [&](const ItemGeo &g, int t) -> KeySteps {
         const int k0 = (g.t0 + t) * RW_KT;
@@ -252,19 +398,39 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
         }
         __syncwarp();
     };
-    // a tile of keys that some row of the item does not see whole
-    auto masked = [&](const ItemGeo &g, int t) -> bool {
-        const int k0 = (g.t0 + t) * RW_KT;
-        return k0 + RW_KT - 1 > g.pmin || (a.window > 0 && k0 < g.pmax - a.window + 1);
-    };
-
     if (sc.share.n == 0) {
         // no share
     } else if (warp == 8) {
-        // ---- K and V tiles ----
-        PlanWalk<RW_R, RW_KT> w(a, sc.share);
-        int it = 0, item = 0, fills[2] = {0, 0};
-        bool ok = true;
+        // ---- items; Q, K and V tiles ----
+        PlanWalk<RW_R, RW_KT> walk(a, sc.share);
+        ItemDesc w, next;
+        int it = 0, item = 0, left = 0, fills[2] = {0, 0};
+        bool ok = true, more = walk.load();
+        auto leave = [&]() {  // the item of the walk, or the end, for the other warps
+            next.th = next.tl = 0;
+            if (more) {
+                next.g = walk.g;
+                next.b = walk.b;
+                next.kvh = walk.kvh;
+                next.q0 = walk.s.q0;
+                next.p0 = walk.s.p0;
+                next.tl = walk.tl;
+                next.th = walk.th;
+                next.k0 = -1;
+                if (!walk.whole()) {
+                    const CutItem c = cut_item(walk);
+                    next.k0 = c.k0;
+                    next.k1 = c.k1;
+                }
+            }
+            if (left >= RW_ITEMS) ok = ok && wait_all(&bar.d_free[left % RW_ITEMS], (left / RW_ITEMS - 1) & 1);
+            if (lane == 0) {
+                items[left % RW_ITEMS] = next;
+                mbar_arrive(&bar.d_full[left % RW_ITEMS]);
+            }
+            ++left;
+            __syncwarp();
+        };
         auto load_q = [&]() {
             for (int t = 0; t < 2; ++t) {
                 const int b = item % QB * 2 + t;
@@ -273,11 +439,16 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 __syncwarp();
                 if (lane < C::PANELS)
                     tma_load_3d(qs + b * C::TILE + lane * 16384, &qmap, &bar.q_full[b], lane * 64, w.kvh * a.G,
-                                w.s.q0 + div_g(a, w.g.r0 + t * 128));
+                                w.q0 + div_g(a, w.g.r0 + t * 128));
                 __syncwarp();
             }
         };
-        for (bool more = w.load(); more && ok; more = w.next(), ++item) {
+        leave();
+        for (; more && ok; ++item) {
+            w = next;
+            more = walk.next();
+            leave();
+            if (!ok) break;
             if (qtma && QB > 1) load_q();
             for (int t = w.tl; t < w.th && ok; ++t, ++it) {
                 // one Q buffer: the item's first K and V need not wait for it
@@ -307,7 +478,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                             const int page = a.table[(int64_t)w.b * a.max_pages + key / a.page_size];
                             tma_load_4d(d, map, full, p * 64, key % a.page_size, w.kvh, page);
                         } else {
-                            tma_load_3d(d, map, full, p * 64, w.s.q0 + key, w.kvh);
+                            tma_load_3d(d, map, full, p * 64, w.q0 + key, w.kvh);
                         }
                     }
                     __syncwarp();
@@ -333,11 +504,11 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
         constexpr uint32_t ID = (1u << 4) | (E::FMT << 7) | (E::FMT << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
         const uint32_t tmu = uniform(tm);
         const uint64_t qd0 = sw128_desc(qs), kd0 = sw128_desc(ks);
-        PlanWalk<RW_R, RW_KT> w(a, sc.share);
+        ItemDesc w;
         int n = 0, sbuf = 0, qbuf = 0, kst = 0;
         uint32_t qph = 0, kph = 0;
         bool ok = true;
-        for (bool more = w.load(); more && ok; more = w.next()) {
+        for (int item = 0; ok && take(item, w, ok); ++item) {
             const int left = uniform(w.th - w.tl);
             for (int j = 0; j < left && ok; ++j) {
 #pragma unroll
@@ -378,11 +549,11 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                                 ((128u >> 4) << 24);
         const uint32_t tmu = uniform(tm);
         const uint64_t vd0 = sw128_desc_n(smem_u32(vs), 16384);
-        PlanWalk<RW_R, RW_KT> w(a, sc.share);
+        ItemDesc w;
         int n = 0, pbuf = 0, vst = 0;
         uint32_t pph = 0, vph = 0;
         bool ok = true;
-        for (bool more = w.load(); more && ok; more = w.next()) {
+        for (int item = 0; ok && take(item, w, ok); ++item) {
             const int left = uniform(w.th - w.tl);
             for (int j = 0; j < left && ok; ++j) {
                 const KeySteps ks_ = key_steps(w.g, w.tl + j);
@@ -418,12 +589,12 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
         drain(ok, &bar.drain[1]);
     } else if (warp == 10) {
         // ---- Q rows; V rows of masked tiles ----
-        PlanWalk<RW_R, RW_KT> w(a, sc.share), wn(a, sc.share);  // the item at hand, the next one
-        constexpr int CH = C::PANELS * 8, STEP = 32 / CH;       // 16-byte pieces of a row, rows at a time
+        ItemDesc w, wn = {};                               // the item at hand, the next one
+        constexpr int CH = C::PANELS * 8, STEP = 32 / CH;  // 16-byte pieces of a row, rows at a time
         const int c = lane % CH;
         const bool col = c * 8 < a.D;
         auto load_q = [&](int item) {
-            const T *q = reinterpret_cast<const T *>(a.q) + (int64_t)wn.s.q0 * a.qs[0] + (int64_t)wn.kvh * a.G * a.qs[1] + c * 8;
+            const T *q = reinterpret_cast<const T *>(a.q) + (int64_t)wn.q0 * a.qs[0] + (int64_t)wn.kvh * a.G * a.qs[1] + c * 8;
             for (int t = 0; t < 2; ++t) {
                 const uint32_t dst = smem_u32(qs + (item % QB * 2 + t) * C::TILE) + (c / 8) * 16384;
 #pragma unroll 4
@@ -443,9 +614,9 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             if (lane < 2) mbar_arrive(&bar.q_full[item % QB * 2 + lane]);
         };
         int it = 0, item = 0, loaded = 0;  // key tiles and items done, items whose Q is loaded
-        bool ok = true, qmore = wn.load();
+        bool ok = true, qmore = take(0, wn, ok);
         auto q_turn = [&](bool block) -> bool {  // the next item's Q, once its buffer is free
-            if (qtma || !qmore || loaded > item + 1) return true;
+            if (qtma || !qmore || loaded > item) return true;
             for (int t = 0; t < 2 && loaded >= QB; ++t) {
                 uint64_t *b = &bar.q_free[loaded % QB * 2 + t];
                 const uint32_t ph = (loaded / QB - 1) & 1;
@@ -456,47 +627,62 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 }
             }
             load_q(loaded++);
-            qmore = wn.next();
             return true;
         };
-        ok = q_turn(true);
-        for (bool more = w.load(); more && ok; more = w.next(), ++item) {
+        // `item`: the one whose Q comes next, wn
+        ok = ok && q_turn(true);
+        while (qmore && ok) {
+            w = wn;
+            const int at = item++;
+            qmore = take(item, wn, ok);
             for (int t = w.tl; t < w.th && ok; ++t, ++it) {
                 const int s = it % NS;
                 if (!(ok = q_turn(false)) || !(ok = wait_all(&bar.v_full[s], (it / NS) & 1))) break;
-                if (masked(w.g, t)) {
+                if (rows_masked(w.g, t, a.window)) {
                     const int k0 = (w.g.t0 + t) * RW_KT;
                     const KeySteps st = key_steps(w.g, t);
                     uint8_t *v = vs + s * C::TILE;
-                    bool bad = false;
-                    // rows that the products read and some row of the item does not see: before a, from b on
-                    const int a0 = max(w.g.kb, a.window > 0 ? w.g.pmax - a.window + 1 : 0) - k0, b0 = w.g.pmin + 1 - k0;
-                    const int ra = min(max(a0, st.lo * 16), st.hi * 16), rb = min(max(b0, ra), st.hi * 16);
-                    for (int r = st.lo * 16 + lane / 8; r < st.hi * 16; r += 4) {
-                        if (r >= ra && r < rb) continue;
-                        const bool out = k0 + r < w.g.kb || k0 + r >= w.g.ke;
+                    const int lo = st.lo * 16, hi = st.hi * 16;  // rows that the products read
+                    const int kb = min(max(w.g.kb - k0, lo), hi), ke = min(max(w.g.ke - k0, kb), hi);  // those of the item's keys
+                    // of those, the ones that every row sees
+                    const int a0 = min(max(a.window > 0 ? w.g.pmax - a.window + 1 - k0 : kb, kb), ke);
+                    const int b0 = min(max(w.g.pmin + 1 - k0, a0), ke);
+                    auto clear = [&](int from, int to) {
+                        for (int r = from + lane / 8; r < to; r += 4)
 #pragma unroll
-                        for (int p = 0; p < C::PANELS; ++p) {
-                            uint4 *q = reinterpret_cast<uint4 *>(v + p * 16384 + r * 128) + lane % 8;
-                            if (out) {
-                                *q = make_uint4(0, 0, 0, 0);
-                                continue;
-                            }
-                            const uint4 x = *q;
-                            uint32_t e[4] = {x.x, x.y, x.z, x.w};
-                            bool hit = false;
+                            for (int p = 0; p < C::PANELS; ++p)
+                                *(reinterpret_cast<uint4 *>(v + p * 16384 + r * 128) + lane % 8) = make_uint4(0, 0, 0, 0);
+                    };
+                    clear(lo, kb);
+                    clear(ke, hi);
+                    // is an exponent all ones: adding its lowest bit carries into the sign's place
+                    uint32_t acc = 0;
+                    auto look = [&](int from, int to) {
+#pragma unroll 4
+                        for (int r = from + lane / 8; r < to; r += 4)
 #pragma unroll
-                            for (int m = 0; m < 4; ++m) {
-                                const bool lo = (e[m] & E::EXP) == E::EXP, hi = (e[m] >> 16 & E::EXP) == E::EXP;
-                                if (lo) e[m] &= 0xFFFF0000u;
-                                if (hi) e[m] &= 0x0000FFFFu;
-                                hit |= lo | hi;
+                            for (int p = 0; p < C::PANELS; ++p) {
+                                const uint4 x = *(reinterpret_cast<const uint4 *>(v + p * 16384 + r * 128) + lane % 8);
+                                constexpr uint32_t M = E::EXP * 0x10001u, ONE = (E::EXP & (0u - E::EXP)) * 0x10001u;
+                                acc |= (x.x & M) + ONE | (x.y & M) + ONE | (x.z & M) + ONE | (x.w & M) + ONE;
                             }
-                            if (hit) *q = make_uint4(e[0], e[1], e[2], e[3]);
-                            bad |= hit;
+                    };
+                    look(kb, a0);
+                    look(b0, ke);
+                    const bool bad = __any_sync(0xffffffffu, (acc & 0x80008000u) != 0);
+                    if (bad)
+                        for (int r = kb + lane / 8; r < ke; r += 4) {
+                            if (r >= a0 && r < b0) continue;
+#pragma unroll 1
+                            for (int p = 0; p < C::PANELS * 4; ++p) {
+                                uint32_t *q = reinterpret_cast<uint32_t *>(v + p / 4 * 16384 + r * 128 + lane % 8 * 16) + p % 4;
+                                uint32_t x = *q;
+                                if ((x & E::EXP) == E::EXP) x &= 0xFFFF0000u;
+                                if ((x >> 16 & E::EXP) == E::EXP) x &= 0x0000FFFFu;
+                                *q = x;
+                            }
                         }
-                    }
-                    if (bad) odd[item & 3] = item + 1;
+                    if (bad && lane == 0) odd[at & 3] = at + 1;
                     fence_async_smem();
                 }
                 mbar_arrive(&bar.v_fixed[s]);
@@ -508,7 +694,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
         const int t = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, ot = tm + lanes + C::O0 + t * HD;
         const float c = __fmul_rn(a.scale, 1.4426950408889634f);
-        PlanWalk<RW_R, RW_KT> w(a, sc.share);
+        ItemDesc w;
         int it = 0, item = 0;  // key tiles and items done
         uint32_t both_n = 0;
         bool ok = true;
@@ -524,10 +710,10 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             tc_fence_after();
             return done;
         };
-        for (bool more = w.load(); more && ok; more = w.next(), ++item) {
-            const ItemGeo g = w.g;
+        for (; ok && take(item, w, ok); ++item) {
+            const ItemGeo &g = w.g;
             const int f = g.r0 + t * 128 + r, tok = div_g(a, f);
-            const int pos = f < g.r1 ? w.s.p0 + tok : -1;
+            const int pos = f < g.r1 ? w.p0 + tok : -1;
             const float sink = a.sinks && f < g.r1 ? __fmul_rn(a.sinks[w.kvh * a.G + f - tok * a.G], 1.4426950408889634f) : 0.0f;
             // positions of the warp's rows, lowest and highest
             const int plo = __reduce_min_sync(0xffffffffu, pos < 0 && f >= g.r1 ? INT_MAX : pos),
@@ -555,7 +741,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                     const float nmc = __fsub_rn(E::BIAS, mr);
                     const uint64_t nmc2 = f2_pack(nmc, nmc);
                     tmem_ld32(st, sv);
-#pragma unroll 1
+#pragma unroll(HD == 128 ? 2 : 1)
                     for (; xs < 4; ++xs) {
                         uint64_t v[16], part[2] = {0, 0};
                         uint32_t pk[16];
@@ -606,26 +792,8 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                         l = __fmul_rn(l, corr);
                         sum[0] = f2_mul(sum[0], f2_pack(corr, corr));
                         sum[1] = f2_mul(sum[1], f2_pack(corr, corr));
-#pragma unroll 1
-                        for (int x = 0; x < HD; x += 16) {
-                            uint32_t ov[16];
-                            tmem_ld16(ot + x, ov);
-                            tmem_ld_wait16(ov);
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) ov[y] = __float_as_uint(__fmul_rn(__uint_as_float(ov[y]), corr));
-                            tmem_st16(ot + x, ov);
-                        }
-                        tmem_st_wait();
-#pragma unroll 1
-                        for (int x = 0; x < 16 * xs; x += 16) {  // weights of this tile that are written: exact, corr is a power of two
-                            uint32_t ov[16];
-                            tmem_ld16(st + x, ov);
-                            tmem_ld_wait16(ov);
-#pragma unroll
-                            for (int y = 0; y < 16; ++y)
-                                ov[y] = E::pack(__fmul_rn(E::up(ov[y] & 0xFFFFu), corr), __fmul_rn(E::up(ov[y] >> 16), corr));
-                            tmem_st16(st + x, ov);
-                        }
+                        scale_o(ot, HD, corr);
+                        if (xs) scale_p<T>(st, 16 * xs, corr);
                     }
                     const float nmc = mr == -INFINITY ? 0.0f : __fsub_rn(E::BIAS, mr);
                     const uint64_t nmc2 = f2_pack(nmc, nmc);
@@ -657,85 +825,29 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             }
             if (!ok || !(ok = o_done())) break;
             float mref = mr;
-            // 32 columns of this block's O, with what masked tiles hold of non-finite V for the rows that see it
-            auto own_o = [&](int x, float (&o)[32]) {
-                uint32_t ov[32];
-                tmem_ld32(ot + x, ov);
-                tmem_ld_wait32(ov);
-#pragma unroll
-                for (int d = 0; d < 32; ++d) o[d] = __uint_as_float(ov[d]);
-                if (odd[item & 3] != item + 1) return;
-                const T *vb = reinterpret_cast<const T *>(a.v) + (int64_t)w.kvh * a.vs[2];
-                for (int key = (g.t0 + w.tl) * RW_KT; key < (g.t0 + w.th) * RW_KT; ++key) {
-                    if (key < g.kb || key >= g.ke || key > pos || (a.window > 0 && key <= pos - a.window) ||
-                        !masked(g, key / RW_KT - g.t0))
-                        continue;
-                    const T *vp = vb + (int64_t)(w.s.q0 + key) * a.vs[1];
-                    if (a.table) {
-                        const int page = a.table[(int64_t)w.b * a.max_pages + key / a.page_size];
-                        if (page < 0 || page >= a.n_pages) continue;
-                        vp = vb + page * a.vs[0] + (int64_t)(key % a.page_size) * a.vs[1];
-                    }
-#pragma unroll
-                    for (int d = 0; d < 32; ++d) {
-                        const float v = x + d < a.D ? E::up(reinterpret_cast<const unsigned short *>(vp)[x + d]) : 0.0f;
-                        if (!isfinite(v)) o[d] = __fadd_rn(o[d], v);
-                    }
-                }
-            };
-            const bool cut = !w.whole();
-            CutItem ci = {0, 0};
-            if (cut) {
-                ci = cut_item(w);
-                float *mine = a.part + ((int64_t)blockIdx.x * 2 + (w.tl == 0)) * C::PART + tid;
-#pragma unroll 1
-                for (int x = 0; x < HD; x += 32) {
-                    float o[32];
-                    own_o(x, o);
-#pragma unroll
-                    for (int d = 0; d < 32; ++d) __stcg(mine + (x + d) * RW_R, o[d]);
-                }
-                __stcg(mine + HD * RW_R, mref);
-                __stcg(mine + (HD + 1) * RW_R, l);
+            if (odd[item & 3] == item + 1) add_odd<T, HD>(a, w, pos, ot);
+            if (w.k0 >= 0) {
+                leave_part<HD>(a.part + ((int64_t)blockIdx.x * 2 + (w.tl == 0)) * C::PART + tid, ot, mref, l);
                 __threadfence();
                 if (!(ok = both())) break;
                 if (tid == 0) {
-                    lastf = atomicAdd(a.ticket + ci.k0, 1u) == (unsigned)(ci.k1 - ci.k0);
-                    if (lastf) a.ticket[ci.k0] = 0u;
+                    lastf = atomicAdd(a.ticket + w.k0, 1u) == (unsigned)(w.k1 - w.k0);
+                    if (lastf) a.ticket[w.k0] = 0u;
                 }
                 if (!(ok = both())) break;
                 if (!lastf) continue;
                 __threadfence();
-                float mm = -INFINITY;
-                for (int k = ci.k0; k <= ci.k1; ++k)
-                    mm = fmaxf(mm, __ldcg(a.part + ((int64_t)k * 2 + (k == ci.k0)) * C::PART + HD * RW_R + tid));
-                const float ms = mm == -INFINITY ? 0.0f : mm;
-                l = 0.0f;
-                for (int k = ci.k0; k <= ci.k1; ++k) {
-                    const float *p = a.part + ((int64_t)k * 2 + (k == ci.k0)) * C::PART + HD * RW_R + tid;
-                    l = __fmaf_rn(__ldcg(p + RW_R), ex2(__fsub_rn(__ldcg(p), ms)), l);
-                }
-                mref = mm;
+                const float2 ml = join_parts<HD>(a.part + tid, w.k0, w.k1, ot);
+                mref = ml.x;
+                l = ml.y;
             }
             const float inv = f < g.r1 ? row_factor<E>(mref, l, a.sinks != nullptr, sink) : 0.0f;
-            T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.s.q0 + tok) * a.os[0] + (int64_t)(w.kvh * a.G + f - tok * a.G) * a.os[1];
+            T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.q0 + tok) * a.os[0] + (int64_t)(w.kvh * a.G + f - tok * a.G) * a.os[1];
 #pragma unroll 1
             for (int x = 0; x < HD; x += 32) {
-                float o[32];
-                if (!cut) {
-                    own_o(x, o);
-                } else {
-                    const float ms = mref == -INFINITY ? 0.0f : mref;
-#pragma unroll
-                    for (int d = 0; d < 32; ++d) o[d] = 0.0f;
-#pragma unroll 1
-                    for (int k = ci.k0; k <= ci.k1; ++k) {
-                        const float *p = a.part + ((int64_t)k * 2 + (k == ci.k0)) * C::PART + tid;
-                        const float e = ex2(__fsub_rn(__ldcg(p + HD * RW_R), ms));
-#pragma unroll
-                        for (int d = 0; d < 32; ++d) o[d] = __fmaf_rn(__ldcg(p + (x + d) * RW_R), e, o[d]);
-                    }
-                }
+                uint32_t o[32];
+                tmem_ld32(ot + x, o);
+                tmem_ld_wait32(o);
                 if (f < g.r1)
 #pragma unroll
                     for (int ch = 0; ch < 4; ++ch)
@@ -743,7 +855,8 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                             uint32_t e[4];
 #pragma unroll
                             for (int y = 0; y < 4; ++y)  // a row without keys: 0 x 0
-                                e[y] = E::pack(__fmul_rn(o[ch * 8 + 2 * y], inv), __fmul_rn(o[ch * 8 + 2 * y + 1], inv));
+                                e[y] = E::pack(__fmul_rn(__uint_as_float(o[ch * 8 + 2 * y]), inv),
+                                               __fmul_rn(__uint_as_float(o[ch * 8 + 2 * y + 1]), inv));
                             *reinterpret_cast<uint4 *>(out + x + ch * 8) = make_uint4(e[0], e[1], e[2], e[3]);
                         }
             }
