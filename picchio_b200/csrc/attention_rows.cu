@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                     // is an exponent all ones: adding its lowest bit carries into the sign's place
                     uint32_t acc = 0;
                     auto look = [&](int from, int to) {
-#pragma unroll 4
+#pragma unroll 1
                         for (int r = from + lane / 8; r < to; r += 4)
 #pragma unroll
                             for (int p = 0; p < C::PANELS; ++p) {
