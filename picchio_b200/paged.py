@@ -11,6 +11,7 @@ device unless ``stream`` is given, and waits for nothing.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 from .api import _check, lib
@@ -40,6 +41,13 @@ class _Call(C.Structure):
                 ("window", C.c_int), ("scale", C.c_float)]
 
 
+# The same as bytes, which are made in a quarter of a ctypes structure's time:
+# the smallest calls are as long as their Python side.
+_pages_bytes, _step_bytes, _call_bytes = (struct.Struct("@" + f) for f in ("2P6q5i0P", "5i11P", "P2qP2q6i2Pif0P"))
+_two_bytes = struct.Struct("@2q").pack
+assert [f.size for f in (_pages_bytes, _step_bytes, _call_bytes)] == [C.sizeof(t) for t in (_Pages, _Step, _Call)]
+
+
 class StepTables(NamedTuple):
     """What :func:`kv_tables` returns; int32 except ``slots`` (int64)."""
     kv_len: object     # [B] lengths after the step
@@ -54,8 +62,6 @@ _L = None
 _dt = {}           # torch dtype -> PC_DT_*
 _i32 = _i64 = None  # torch.int32, torch.int64
 _raw_stream = None  # device index -> handle of torch's current stream
-_Two = C.c_int64 * 2
-_byref = C.byref
 
 
 def _entry():
@@ -63,14 +69,14 @@ def _entry():
     if _L is None:
         import torch
         L = lib()
-        vp, i64p = C.c_void_p, C.POINTER(C.c_int64)
-        L.pc_kv_tables.argtypes = [C.c_int, C.POINTER(_Step), vp]
-        L.pc_kv_store.argtypes = [C.c_int, C.POINTER(_Pages), vp, i64p, vp, i64p, C.c_int, vp, C.c_int, vp]
+        vp = C.c_void_p  # structures and strides go as bytes
+        L.pc_kv_tables.argtypes = [C.c_int, vp, vp]
+        L.pc_kv_store.argtypes = [C.c_int, vp, vp, vp, vp, vp, C.c_int, vp, C.c_int, vp]
         L.pc_attn_create.argtypes = [C.c_int, C.POINTER(vp)]
         L.pc_attn_free.argtypes = [vp]
         L.pc_attn_free.restype = None
-        L.pc_attn_paged.argtypes = [vp, C.POINTER(_Call), C.POINTER(_Pages), vp, C.c_int, vp, vp]
-        L.pc_attn_packed.argtypes = [vp, C.POINTER(_Call), vp, i64p, vp, i64p, vp]
+        L.pc_attn_paged.argtypes = [vp, vp, vp, vp, C.c_int, vp, vp]
+        L.pc_attn_packed.argtypes = [vp, vp, vp, vp, vp, vp, vp]
         L.pc_attn_check.argtypes = [vp, vp]
         for n in ("pc_kv_tables", "pc_kv_store", "pc_attn_create", "pc_attn_paged", "pc_attn_packed",
                   "pc_attn_check"):
@@ -87,6 +93,15 @@ def _entry():
 def _stream(dev, stream):
     """The stream of a call on device `dev`: torch's current one unless given."""
     return _raw_stream(dev) if stream is None else getattr(stream, "cuda_stream", stream)
+
+
+def _made(t, stream):
+    """A tensor made for a call on `stream`: torch does not hand its memory
+    out again before that stream is done with it."""
+    if stream is not None:
+        import torch
+        t.record_stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream, t.device))
+    return t
 
 
 def _type(t, name):
@@ -111,15 +126,17 @@ def _heads3(t, name, dev):
     return shape, st
 
 
-def _pages(k_pages, v_pages, dev) -> _Pages:
+def _pages(k_pages, v_pages, dev):
+    """(bytes of the pc_kv_pages, KV heads, head_dim)"""
     shape = k_pages.shape
     ks, vs = k_pages.stride(), v_pages.stride()
     if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype or k_pages.get_device() != dev \
             or v_pages.get_device() != dev or ks[3] != 1 or vs[3] != 1:
         raise ValueError(f"k_pages, v_pages: two tensors [pages, page_size, kv_heads, head_dim] of one type on cuda:{dev} "
                          "with contiguous head_dim expected")
-    return _Pages(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                  _type(k_pages, "k_pages"), shape[0], shape[1], shape[2], shape[3])
+    n, page, heads, dim = shape
+    return _pages_bytes.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                             _type(k_pages, "k_pages"), n, page, heads, dim), heads, dim
 
 
 def kv_tables(kv_len, new_len, page_table, free_pages, n_free, *, page_size: int, n_tokens: int, stream=None) -> StepTables:
@@ -136,18 +153,21 @@ def kv_tables(kv_len, new_len, page_table, free_pages, n_free, *, page_size: int
     if dev < 0 or page_table.shape != (B, width) or n_tokens < 0:
         raise ValueError("kv_len on a CUDA device, page_table [requests, max_pages] and n_tokens >= 0 expected")
     cap = free_pages.numel()
-    ptrs = (_ints(kv_len, "kv_len", dev, B, _i32), _ints(new_len, "new_len", dev, B, _i32),
-            _ints(n_free, "n_free", dev, 1, _i32), _ints(page_table, "page_table", dev, B * width, _i32),
-            _ints(free_pages, "free_pages", dev, cap, _i32))
+    if not (kv_len.dtype is new_len.dtype is page_table.dtype is free_pages.dtype is n_free.dtype is _i32
+            and new_len.get_device() == page_table.get_device() == free_pages.get_device() == n_free.get_device() == dev
+            and new_len.numel() == B and n_free.numel() == 1 and kv_len.is_contiguous() and new_len.is_contiguous()
+            and page_table.is_contiguous() and free_pages.is_contiguous()):
+        raise ValueError(f"kv_len, new_len [{B}], page_table, free_pages, n_free [1]: contiguous int32 tensors on cuda:{dev} expected")
     # one allocation: cu_new, kv_end, served, n_free, positions
-    buf = kv_len.new_empty(3 * B + 2 + n_tokens)
-    slots = kv_len.new_empty(n_tokens, dtype=_i64)
+    buf = _made(kv_len.new_empty(3 * B + 2 + n_tokens), stream)
+    slots = _made(kv_len.new_empty(n_tokens, dtype=_i64), stream)
     base = buf.data_ptr()
     end = base + 4 * (B + 1)
     served = end + 4 * B
-    s = _Step(B, width, page_size, n_tokens, cap, *ptrs, end, base, served, served + 4 * B, served + 4 * B + 4,
-              slots.data_ptr())
-    _check(L.pc_kv_tables(dev, _byref(s), _stream(dev, stream)))
+    s = _step_bytes.pack(B, width, page_size, n_tokens, cap, kv_len.data_ptr(), new_len.data_ptr(), n_free.data_ptr(),
+                         page_table.data_ptr(), free_pages.data_ptr(), end, base, served, served + 4 * B,
+                         served + 4 * B + 4, slots.data_ptr())
+    _check(L.pc_kv_tables(dev, s, _stream(dev, stream)))
     cu, end, served, left, pos = buf.split_with_sizes((B + 1, B, B, 1, n_tokens))
     return StepTables(end, cu, served, left, pos, slots)
 
@@ -160,12 +180,12 @@ def kv_store(k_pages, v_pages, k, v, slots, stream=None) -> None:
     dev, n = k.get_device(), slots.numel()
     if dev < 0:
         raise ValueError("k: a CUDA tensor expected")
-    p = _pages(k_pages, v_pages, dev)
+    p, heads, dim = _pages(k_pages, v_pages, dev)
     shape, ks = _heads3(k, "k", dev)
     vshape, vs = _heads3(v, "v", dev)
-    if shape != vshape or k.dtype is not v.dtype or shape != (n, p.n_kv_heads, p.head_dim):
-        raise ValueError(f"k and v: two tensors [{n}, {p.n_kv_heads}, {p.head_dim}] of one type expected")
-    _check(L.pc_kv_store(dev, _byref(p), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
+    if shape != vshape or k.dtype is not v.dtype or shape != (n, heads, dim):
+        raise ValueError(f"k and v: two tensors [{n}, {heads}, {dim}] of one type expected")
+    _check(L.pc_kv_store(dev, p, k.data_ptr(), _two_bytes(ks[0], ks[1]), v.data_ptr(), _two_bytes(vs[0], vs[1]),
                          _type(k, "k"), _ints(slots, "slots", dev, n, _i64), n, _stream(dev, stream)))
 
 
@@ -178,25 +198,27 @@ class Attention:
         _check(_entry().pc_attn_create(device, C.byref(h)))
         self._h, self.device = h, device
 
-    def _call(self, q, cu_new, sinks, window, scale, kv_heads, out):
+    def _call(self, q, cu_new, sinks, window, scale, kv_heads, out, stream):
+        """(bytes of the pc_attn_call, out, requests)"""
         dev = self.device
         shape, qs = _heads3(q, "q", dev)
         T, H, D = shape
         if out is None:
-            out = q.new_empty(shape)
+            out = _made(q.new_empty(shape), stream)
             os = (H * D, D)
         else:
             oshape, os = _heads3(out, "out", dev)
             if oshape != shape or out.dtype is not q.dtype:
                 raise ValueError("out: a tensor like q expected")
-        sp = None
+        sp = 0
         if sinks is not None:
             if _dt.get(sinks.dtype) != DT_F32 or sinks.numel() != H or sinks.get_device() != dev or not sinks.is_contiguous():
                 raise ValueError(f"sinks: a contiguous float32 tensor of {H} elements on cuda:{dev} expected")
             sp = sinks.data_ptr()
         n = cu_new.numel()
-        return _Call(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], _type(q, "q"), H, kv_heads, D, T, n - 1,
-                     _ints(cu_new, "cu_new", dev, n, _i32), sp, int(window), D ** -0.5 if scale is None else scale), out
+        return _call_bytes.pack(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], _type(q, "q"), H, kv_heads, D, T,
+                                n - 1, _ints(cu_new, "cu_new", dev, n, _i32), sp, int(window),
+                                D ** -0.5 if scale is None else scale), out, n - 1
 
     def paged(self, q, k_pages, v_pages, page_table, cu_new, kv_len, *, sinks=None, window: int = 0, scale=None,
               out=None, stream=None):
@@ -208,12 +230,12 @@ class Attention:
         ``kv_len`` [B] int32: positions in the cache, the new rows' included.
         """
         dev = self.device
-        p = _pages(k_pages, v_pages, dev)
-        c, out = self._call(q, cu_new, sinks, window, scale, p.n_kv_heads, out)
-        B, width = c.n_requests, page_table.shape[-1]
+        p, heads, _ = _pages(k_pages, v_pages, dev)
+        c, out, B = self._call(q, cu_new, sinks, window, scale, heads, out, stream)
+        width = page_table.shape[-1]
         if page_table.shape != (B, width):
             raise ValueError(f"page_table: [{B}, max_pages] expected")
-        _check(_L.pc_attn_paged(self._h, _byref(c), _byref(p), _ints(page_table, "page_table", dev, B * width, _i32), width,
+        _check(_L.pc_attn_paged(self._h, c, p, _ints(page_table, "page_table", dev, B * width, _i32), width,
                                 _ints(kv_len, "kv_len", dev, B, _i32), _stream(dev, stream)))
         return out
 
@@ -224,11 +246,12 @@ class Attention:
         dev = self.device
         shape, ks = _heads3(k, "k", dev)
         vshape, vs = _heads3(v, "v", dev)
-        c, out = self._call(q, cu_new, sinks, window, scale, shape[1], out)
-        if shape != vshape or k.dtype is not q.dtype or v.dtype is not q.dtype or shape[0] != c.n_rows or shape[2] != c.head_dim:
+        c, out, _ = self._call(q, cu_new, sinks, window, scale, shape[1], out, stream)
+        T, _, D = q.shape
+        if shape != vshape or k.dtype is not q.dtype or v.dtype is not q.dtype or shape[0] != T or shape[2] != D:
             raise ValueError("k and v: [rows, kv_heads, head_dim] of q's rows, head_dim and type expected")
-        _check(_L.pc_attn_packed(self._h, _byref(c), k.data_ptr(), _Two(ks[0], ks[1]), v.data_ptr(), _Two(vs[0], vs[1]),
-                                 _stream(dev, stream)))
+        _check(_L.pc_attn_packed(self._h, c, k.data_ptr(), _two_bytes(ks[0], ks[1]), v.data_ptr(),
+                                 _two_bytes(vs[0], vs[1]), _stream(dev, stream)))
         return out
 
     def check(self, stream=None):
