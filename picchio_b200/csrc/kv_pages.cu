@@ -15,7 +15,13 @@ namespace {
 
 constexpr int TAB_THREADS = 1024;
 
-// Inclusive sums over the block of three values at once.
+// Sums stop here (adding so stays associative): 1024 requests can ask for more
+// than 32 bits hold, and whatever is above every capacity is refused alike.
+// Capacities and single values are at most half of it.
+constexpr int TAB_MOST = 1 << 29;
+__device__ __forceinline__ int add_most(int a, int b) { return min(a + b, TAB_MOST); }
+
+// Inclusive sums over the block of three values at once, none below zero.
 __device__ __forceinline__ void block_scan3(int (&v)[3], int (&all)[3], int (*sh)[TAB_THREADS / 32]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -23,7 +29,7 @@ __device__ __forceinline__ void block_scan3(int (&v)[3], int (&all)[3], int (*sh
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v[c], o);
-            if (lane >= o) v[c] += u;
+            if (lane >= o) v[c] = add_most(v[c], u);
         }
     __syncthreads();
     if (lane == 31)
@@ -32,15 +38,15 @@ __device__ __forceinline__ void block_scan3(int (&v)[3], int (&all)[3], int (*sh
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
-        const int x = sh[c][lane];
-        int inc = x;
+        int inc = sh[c][lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
+            if (lane >= o) inc = add_most(inc, u);
         }
         all[c] = __shfl_sync(0xffffffffu, inc, 31);
-        v[c] += __shfl_sync(0xffffffffu, inc - x, warp);
+        const int before = __shfl_sync(0xffffffffu, inc, (warp + 31) & 31);
+        if (warp) v[c] = add_most(v[c], before);
     }
 }
 
@@ -103,7 +109,7 @@ __global__ void __launch_bounds__(TAB_THREADS) kv_tables_kernel(const pc_kv_step
         each(b, n, n_free + given + v[0] - n, [&](int r, int j, int at) {
             if (at < s.free_cap) s.free_pages_dev[at] = s.page_table_dev[(int64_t)r * s.max_pages + j];
         });
-        given = (int)min((int64_t)given + all[0], (int64_t)1 << 30);
+        given = add_most(given, all[0]);
     }
     const int avail = min(n_free + given, s.free_cap);
     __syncthreads();
@@ -124,12 +130,12 @@ __global__ void __launch_bounds__(TAB_THREADS) kv_tables_kernel(const pc_kv_step
         }
         const int want = v[0];
         block_scan3(v, all, sh);
-        const int64_t upto = (int64_t)want0 + v[0], tokens = (int64_t)add0 + v[1];
+        const int upto = add_most(want0, v[0]), tokens = add_most(add0, v[1]);
         const bool ok = fits && (want == 0 || upto <= avail) && (add == 0 || tokens <= s.n_tokens);
         int u[3] = {ok ? add : 0, ok ? want : 0, 0}, uall[3];
         block_scan3(u, uall, sh);
         // request b's page held + j is the (upto - want + j)-th from the top of the free ones
-        const int first = ok && want ? (int)(upto - want) : 0;
+        const int first = ok && want ? upto - want : 0;
         each(b, ok ? want : 0, first, [&](int r, int j, int nth) {
             const int kept = (max(s.kv_len_dev[r], 0) + P - 1) / P;
             s.page_table_dev[(int64_t)r * s.max_pages + kept + j] = s.free_pages_dev[avail - 1 - nth];
@@ -139,8 +145,8 @@ __global__ void __launch_bounds__(TAB_THREADS) kv_tables_kernel(const pc_kv_step
             s.served_dev[b] = ok;
             s.cu_new_dev[b + 1] = took0 + u[0];
         }
-        want0 = (int)min((int64_t)want0 + all[0], (int64_t)1 << 30);
-        add0 = (int)min((int64_t)add0 + all[1], (int64_t)1 << 30);
+        want0 = add_most(want0, all[0]);
+        add0 = add_most(add0, all[1]);
         took0 += uall[0];
         used += uall[1];
     }

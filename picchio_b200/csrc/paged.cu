@@ -99,7 +99,7 @@ AttnOp op_of(const pc_attn *a, const pc_attn_call *c) {
     o.G = c->n_heads / c->n_kv_heads;
     o.D = c->head_dim;
     o.inv_g = (unsigned)(((1ull << 32) + o.G - 1) / o.G);
-    o.window = c->window;
+    o.window = std::min(c->window, 1 << 30);  // positions are below it; position - window stays in 32 bits
     o.scale = c->scale;
     o.min_q = 1;
     o.max_q = INT_MAX;
@@ -156,8 +156,9 @@ pc_status pc_kv_tables(int device, const pc_kv_step *s, void *stream) {
         return fail(PC_ERR_INVALID_ARG, "bad pc_kv_tables arguments");
     if (s->page_size < 8 || s->page_size % 8 || s->page_size > (1 << 16))
         return fail(PC_ERR_FORMAT, "page_size must be a multiple of 8, at most 65536");
-    if (s->n_requests > (1 << 20) || s->n_tokens > (1 << 28) || (int64_t)s->max_pages * s->page_size > INT_MAX / 2)
-        return fail(PC_ERR_RANGE, "too many requests, tokens or positions");
+    if (s->n_requests > (1 << 20) || s->n_tokens > (1 << 28) || s->free_cap > (1 << 28) ||
+        (int64_t)s->max_pages * s->page_size > INT_MAX / 2)
+        return fail(PC_ERR_RANGE, "too many requests, tokens, free pages or positions");
     if (s->kv_end_dev == s->kv_len_dev || s->n_free_out_dev == s->n_free_dev)
         return fail(PC_ERR_INVALID_ARG, "kv_end and n_free_out must not overlap the inputs");
     OnDevice on(device);

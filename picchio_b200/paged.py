@@ -217,7 +217,7 @@ class Attention:
             sp = sinks.data_ptr()
         n = cu_new.numel()
         return _call_bytes.pack(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], _type(q, "q"), H, kv_heads, D, T,
-                                n - 1, _ints(cu_new, "cu_new", dev, n, _i32), sp, int(window),
+                                n - 1, _ints(cu_new, "cu_new", dev, n, _i32), sp, min(int(window), 0x7fffffff),
                                 D ** -0.5 if scale is None else scale), out, n - 1
 
     def paged(self, q, k_pages, v_pages, page_table, cu_new, kv_len, *, sinks=None, window: int = 0, scale=None,

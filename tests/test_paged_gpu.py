@@ -205,6 +205,14 @@ def test_paged_rows_without_keys_give_zeros(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_windows_beyond_every_position(dtype):
+    """Windows up to the type's largest and past it: all keys, also for rows
+    before position 0."""
+    for window in (1 << 30, 2**31 - 1, 1 << 40):
+        check_paged([(0, 3), (40, 100), (0, 1), (130, 400), (300, 1), (77, 5)], 16, 8, 2, 64, dtype, False, window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_many_requests(dtype):
     reqs = [(1 + (37 * i) % 90, 1 + i % 2) for i in range(700)]
     check_paged([(max(t, n), n) for t, n in reqs], 8, 4, 1, 32, dtype, True, 0)
@@ -463,6 +471,15 @@ def test_tables_refusals_of_requests():
     run_tables([1, 1, 1, 1], [3, 4, 0, 5], 8, 16, 9, 8)                     # rows run out at the last
     run_tables([16, 50, 16, 30], [20, -1, 33, -1], 8, 16, 0, 100)           # served from ended requests' pages
     run_tables([-4, -1], [3, -1], 8, 16, 5, 4)                              # lengths below zero
+
+
+def test_tables_sums_past_32_bits():
+    """1024 requests that together ask for more rows than 32 bits count: none
+    is served, whatever its sum would wrap to."""
+    n = 1 << 21
+    run_tables([0] * 1025, [n + 1] * 1024 + [3], 257, 8192, 1024 * 257 + 1, n)
+    run_tables([0] * 1025, [2] + [n + 1] * 1023 + [3], 257, 8192, 1024 * 257 + 1, n)
+    run_tables([2**31 - 1] * 3 + [1], [2**31 - 1, -1, 1, 1], 4, 16, 3, 4)
 
 
 def test_tables_large_and_mixed():
