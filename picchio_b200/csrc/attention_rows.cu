@@ -25,11 +25,13 @@
 // and spent more time waiting for instructions than issuing them.
 //
 // Any reference within the exponent range gives the same quotient, so a row
-// keeps the one of its first tile, and later tiles are not searched for their
-// maximum first: the sum of 32 weights shows when one has grown past 2^14 (f16
-// weights, stored 2^7 up, end at 2^16), and then the tile is gone through the
-// careful way from there on: maximum, reference moved by a power of two, O and
-// what is written of the tile rescaled.
+// keeps its first one (at head sizes to 64 the maximum of its first 32 scores
+// where all are seen, else that of its first tile), and later scores are not
+// searched for their maximum first: the sum of 32 weights shows when one has
+// grown past 2^14 (f16 weights, stored 2^7 up, end at 2^16), and then the tile
+// is gone through the careful way from there on: maximum, reference moved by a
+// power of two, O and what is written of the tile rescaled.  (Each item's first
+// tile searched whole: 16 prompts 341 us instead of 313.)
 //
 // A key that a row does not see has weight 0, but 0 x NaN is NaN: in tiles
 // that some row does not see whole, V rows outside the item's keys (stale
@@ -42,10 +44,10 @@
 // warps need about 3000 with their waits, instruction fetch among them (loop
 // bodies of more than ~150 instructions, or more code inlined beside them, cost
 // more than they save: unrolling the weights' loop by two took 16 prompts from
-// 338 to 393 us); an item costs about 8000 more.  At head size 128 the two S
+// 338 to 393 us); an item costs about 6000 more.  At head size 128 the two S
 // buffers leave each row tile waiting for its products (2000 of 4300 cycles a
 // tile).  Measured: 16 prompts of 100-2048 tokens, 64 query over 8 KV heads of
-// 64, bf16: 341 us, 468 TFLOP/s; four of 1500-4000 with a window of 128: 150
+// 64, bf16: 313 us, 510 TFLOP/s; four of 1500-4000 with a window of 128: 147
 // us, 1.5 TB/s; one of 8191, 32 over 8 heads of 128, f16: 610 us, 900 TFLOP/s
 // (cuBLAS bf16 1669).
 #include <algorithm>
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             const ItemGeo &g = w.g;
             const int f = g.r0 + t * 128 + r, tok = div_g(a, f);
             const int pos = f < g.r1 ? w.p0 + tok : -1;
-            const float sink = a.sinks && f < g.r1 ? __fmul_rn(a.sinks[w.kvh * a.G + f - tok * a.G], 1.4426950408889634f) : 0.0f;
+            const float sink = a.sinks && f < g.r1 ? a.sinks[w.kvh * a.G + f - tok * a.G] : 0.0f;
             // positions of the warp's rows, lowest and highest
             const int plo = __reduce_min_sync(0xffffffffu, pos < 0 && f >= g.r1 ? INT_MAX : pos),
                       phi = __reduce_max_sync(0xffffffffu, pos);
@@ -747,12 +749,20 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 const uint64_t c2 = f2_pack(c, c);
                 int xs = 0;  // the group from which on the careful way goes
                 bool grown = false;
-                if (all_see(0) && all_see(3) && __all_sync(0xffffffffu, mr != -INFINITY)) {
+                if (all_see(0) && all_see(3) && (HD == 64 || __all_sync(0xffffffffu, mr != -INFINITY))) {
                     // No look at the maximum first: the weights are taken against the reference as it is, and the
                     // sum of a group tells whether one has grown too large for it (or is no number).
+                    tmem_ld32(st, sv);
+                    if (HD == 64 && __any_sync(0xffffffffu, mr == -INFINITY)) {  // none yet: the first group's maximum
+                        float mx = -INFINITY;
+                        tmem_ld_wait32(sv);
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
+                        if (mr == -INFINITY) mr = mx < INFINITY ? __fmul_rn(mx, c) : NAN;
+                    }
                     const float nmc = __fsub_rn(E::BIAS, mr);
                     const uint64_t nmc2 = f2_pack(nmc, nmc);
-                    tmem_ld32(st, sv);
+                    if (HD == 128 || __all_sync(0xffffffffu, mr != -INFINITY))  // else none but -inf so far
 #pragma unroll(HD == 128 ? 2 : 1)
                     for (; xs < 4; ++xs) {
                         uint64_t v[16], part[2] = {0, 0};
@@ -778,56 +788,72 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                     tmem_ld_wait32(sv);
                 }
                 if (xs < 4) {
-                    // the careful way, from group xs on: first tiles, tiles that some row does not see whole
-                    float mx = -INFINITY;
+                    // the careful way, from group xs on: tiles that some row does not see whole; the maximum is searched
+                    // for where a row has no reference yet, or its own has been outgrown
+                    bool search = grown || __any_sync(0xffffffffu, mr == -INFINITY);
+                    do {
+                        if (search) {
+                            float mx = -INFINITY;
 #pragma unroll 1
-                    for (int x = max(x0, xs); x <= x1; ++x) {
-                        tmem_ld32(st + 32 * x, sv);
-                        tmem_ld_wait32(sv);
-                        if (!all_see(x)) hide(sv, seen_bits(lo - 32 * x, hi - 32 * x));
+                            for (int x = max(x0, xs); x <= x1; ++x) {
+                                tmem_ld32(st + 32 * x, sv);
+                                tmem_ld_wait32(sv);
+                                if (!all_see(x)) hide(sv, seen_bits(lo - 32 * x, hi - 32 * x));
 #pragma unroll
-                        for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
-                    }
-                    // move the reference of rows that have none, or whose maximum has grown
-                    const float top = __fmul_rn(mx, c), grow = ceilf(__fsub_rn(top, mr));
-                    float corr = 1.0f;
-                    if (mr == -INFINITY) {
-                        mr = top;
-                    } else if (grow > (grown ? 0.0f : RW_GROW)) {
-                        mr = __fadd_rn(mr, grow);
-                        corr = grow < 126.0f ? __int_as_float((127 - (int)grow) << 23) : 0.0f;
-                    }
-                    if (!(mx < INFINITY)) mr = NAN;  // an infinite or NaN score: so are the row's weights
-                    if (__any_sync(0xffffffffu, corr != 1.0f)) {
-                        ok = o_done();
-                        if (!ok) break;
-                        l = __fmul_rn(l, corr);
-                        sum[0] = f2_mul(sum[0], f2_pack(corr, corr));
-                        sum[1] = f2_mul(sum[1], f2_pack(corr, corr));
-                        scale_o(ot, HD, corr);
-                        if (xs) scale_p<T>(st, 16 * xs, corr);
-                    }
-                    const float nmc = mr == -INFINITY ? 0.0f : __fsub_rn(E::BIAS, mr);
-                    const uint64_t nmc2 = f2_pack(nmc, nmc);
-#pragma unroll 1
-                    for (; xs < 4; ++xs) {
-                        uint32_t pk[16];
-                        if (xs >= x0 && xs <= x1) {
-                            tmem_ld32(st + 32 * xs, sv);
-                            tmem_ld_wait32(sv);
-                            if (!all_see(xs)) hide(sv, seen_bits(lo - 32 * xs, hi - 32 * xs));
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) {
-                                const uint64_t p = f2_ex2(f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2));
-                                sum[y & 1] = f2_add(sum[y & 1], p);
-                                pk[y] = E::pack(f2_lo(p), f2_hi(p));
+                                for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
                             }
-                        } else {
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) pk[y] = 0;
+                            // move the reference of rows that have none, or whose maximum has grown
+                            const float top = __fmul_rn(mx, c), grow = ceilf(__fsub_rn(top, mr));
+                            float corr = 1.0f;
+                            if (mr == -INFINITY) {
+                                mr = top;
+                            } else if (grow > (grown ? 0.0f : RW_GROW)) {
+                                mr = __fadd_rn(mr, grow);
+                                corr = grow < 126.0f ? __int_as_float((127 - (int)grow) << 23) : 0.0f;
+                            }
+                            if (!(mx < INFINITY)) mr = NAN;  // an infinite or NaN score: so are the row's weights
+                            if (__any_sync(0xffffffffu, corr != 1.0f)) {
+                                l = __fmul_rn(l, corr);
+                                sum[0] = f2_mul(sum[0], f2_pack(corr, corr));
+                                sum[1] = f2_mul(sum[1], f2_pack(corr, corr));
+                                if (j > w.tl) {  // O of the tiles before
+                                    ok = o_done();
+                                    if (!ok) break;
+                                    scale_o(ot, HD, corr);
+                                }
+                                if (xs) scale_p<T>(st, 16 * xs, corr);
+                            }
                         }
-                        tmem_st16(st + 16 * xs, pk);
-                    }
+                        const float nmc = mr == -INFINITY ? 0.0f : __fsub_rn(E::BIAS, mr);
+                        const uint64_t nmc2 = f2_pack(nmc, nmc);
+#pragma unroll 1
+                        for (; xs < 4; ++xs) {
+                            uint32_t pk[16];
+                            if (xs >= x0 && xs <= x1) {
+                                uint64_t part[2] = {0, 0};
+                                tmem_ld32(st + 32 * xs, sv);
+                                tmem_ld_wait32(sv);
+                                if (!all_see(xs)) hide(sv, seen_bits(lo - 32 * xs, hi - 32 * xs));
+#pragma unroll
+                                for (int y = 0; y < 16; ++y) {
+                                    const uint64_t p = f2_ex2(f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2));
+                                    part[y & 1] = f2_add(part[y & 1], p);
+                                    pk[y] = E::pack(f2_lo(p), f2_hi(p));
+                                }
+                                part[0] = f2_add(part[0], part[1]);
+                                if (!search && __any_sync(0xffffffffu, !(__fadd_rn(f2_lo(part[0]), f2_hi(part[0])) <= RW_LIMIT))) {
+                                    search = grown = true;
+                                    break;
+                                }
+                                sum[0] = f2_add(sum[0], part[0]);
+                            } else {
+#pragma unroll
+                                for (int y = 0; y < 16; ++y) pk[y] = 0;
+                            }
+                            tmem_st16(st + 16 * xs, pk);
+                        }
+                    } while (xs < 4);
+                    if (!ok) break;
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -853,7 +879,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 mref = ml.x;
                 l = ml.y;
             }
-            const float inv = f < g.r1 ? row_factor<E>(mref, l, a.sinks != nullptr, sink) : 0.0f;
+            const float inv = f < g.r1 ? row_factor<E>(mref, l, a.sinks != nullptr, __fmul_rn(sink, 1.4426950408889634f)) : 0.0f;
             T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.q0 + tok) * a.os[0] + (int64_t)(w.kvh * a.G + f - tok * a.G) * a.os[1];
 #pragma unroll 1
             for (int x = 0; x < HD; x += 32) {

@@ -344,6 +344,41 @@ def test_large_scores(dtype):
         close(out, want, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_keys_of_weight_zero_first(dtype, D):
+    """Scores of -inf for the first 64 positions: as if they were not there."""
+    torch = _torch()
+    q, kp, vp, table, cu, kv = make_paged([(700, 300), (400, 3)], 16, 4, 2, D, dtype, 31)
+    q[..., 0] = 1.0
+    keys = [gathered(kp, table, b, n) for b, n in ((0, 700), (1, 400))]
+    vals = [gathered(vp, table, b, n) for b, n in ((0, 700), (1, 400))]
+    for b in range(2):
+        kp[table[b, :4].long(), :, :, 0] = float("-inf")
+    out = handle().paged(q, kp, vp, table, cu, kv)
+    for b, (total, new) in enumerate([(700, 300), (400, 3)]):
+        want, bound = reference(q[int(cu[b]):int(cu[b + 1])], keys[b][64:], vals[b][64:], total - new - 64, None, 0,
+                                D ** -0.5, dtype)
+        close(out[int(cu[b]):int(cu[b + 1])], want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [0, 150])
+def test_scores_that_grow_late(dtype, window):
+    """A request's last keys outweigh the earlier ones by more than the types'
+    range, within tiles that all rows see and within those that some do not."""
+    torch = _torch()
+    n, H, D = 900, 4, 64
+    g = gen(8)
+    q, k, v = (torch.randn(n, h, D, generator=g, device="cuda") for h in (H, 2, 2))
+    k = k * torch.where(torch.arange(n, device="cuda") % 97 > 80, 4.0, 0.05)[:, None, None]
+    q, k, v = (x.to(_dt(dtype)) for x in (q * 4, k, v))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    out = handle().packed(q, k, v, cu, window=window)
+    want, bound = reference(q, k, v, 0, None, window, D ** -0.5, dtype)
+    close(out, want, bound)
+
+
 def test_same_inputs_same_bits():
     """Items split between blocks are joined in a fixed order."""
     torch = _torch()
