@@ -31,7 +31,7 @@
 // grown past 2^14 (f16 weights, stored 2^7 up, end at 2^16), and then the tile
 // is gone through the careful way from there on: maximum, reference moved by a
 // power of two, O and what is written of the tile rescaled.  (Each item's first
-// tile searched whole: 16 prompts 341 us instead of 313.)
+// tile searched whole: 16 prompts 341 us instead of 312.)
 //
 // A key that a row does not see has weight 0, but 0 x NaN is NaN: in tiles
 // that some row does not see whole, V rows outside the item's keys (stale
@@ -47,7 +47,7 @@
 // 338 to 393 us); an item costs about 6000 more.  At head size 128 the two S
 // buffers leave each row tile waiting for its products (2000 of 4300 cycles a
 // tile).  Measured: 16 prompts of 100-2048 tokens, 64 query over 8 KV heads of
-// 64, bf16: 313 us, 510 TFLOP/s; four of 1500-4000 with a window of 128: 147
+// 64, bf16: 309 us, 516 TFLOP/s; four of 1500-4000 with a window of 128: 145
 // us, 1.5 TB/s; one of 8191, 32 over 8 heads of 128, f16: 610 us, 900 TFLOP/s
 // (cuBLAS bf16 1669).
 #include <algorithm>
@@ -832,8 +832,9 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                             if (xs >= x0 && xs <= x1) {
                                 uint64_t part[2] = {0, 0};
                                 tmem_ld32(st + 32 * xs, sv);
+                                const uint32_t seen = seen_bits(lo - 32 * xs, hi - 32 * xs);
                                 tmem_ld_wait32(sv);
-                                if (!all_see(xs)) hide(sv, seen_bits(lo - 32 * xs, hi - 32 * xs));
+                                hide(sv, seen);
 #pragma unroll
                                 for (int y = 0; y < 16; ++y) {
                                     const uint64_t p = f2_ex2(f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2));
@@ -882,13 +883,13 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
             const float inv = f < g.r1 ? row_factor<E>(mref, l, a.sinks != nullptr, __fmul_rn(sink, 1.4426950408889634f)) : 0.0f;
             T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.q0 + tok) * a.os[0] + (int64_t)(w.kvh * a.G + f - tok * a.G) * a.os[1];
 #pragma unroll 1
-            for (int x = 0; x < HD; x += 32) {
-                uint32_t o[32];
-                tmem_ld32(ot + x, o);
-                tmem_ld_wait32(o);
+            for (int x = 0; x < HD; x += 16) {
+                uint32_t o[16];
+                tmem_ld16(ot + x, o);
+                tmem_ld_wait16(o);
                 if (f < g.r1)
 #pragma unroll
-                    for (int ch = 0; ch < 4; ++ch)
+                    for (int ch = 0; ch < 2; ++ch)
                         if (x + ch * 8 < a.D) {
                             uint32_t e[4];
 #pragma unroll
