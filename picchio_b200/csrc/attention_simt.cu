@@ -11,7 +11,7 @@
 // columns per thread).  The next tile is copied (cp.async) while one is
 // worked on.  Bound by the multiply-adds (128 a cycle and SM) and, at few
 // rows, by the waits of a tile's steps for one another.  Measured, fp32, 64
-// query over 8 KV heads of 64: prompts of 154, 259 and 287 tokens 83 us (the
+// query over 8 KV heads of 64: prompts of 154, 259 and 287 tokens 80 us (the
 // multiply-adds alone 19 us, 25 with the masked ones), three tokens each of 15
 // requests of 173-1430 positions 46 us.
 #include <cuda_bf16.h>
@@ -27,7 +27,7 @@ namespace pc {
 
 namespace {
 
-constexpr int SIMT_KT = 64, SIMT_OV = 32;
+constexpr int SIMT_KT = 64, SIMT_OV = 48;
 
 template <int HDP, int R>
 struct SimtCfg {
@@ -36,6 +36,9 @@ struct SimtCfg {
     static constexpr int KPT = SIMT_KT / TX;      // keys per thread
     static constexpr int DPT = HDP / TX;          // output columns per thread: CV at a time, CV * TX apart
     static constexpr int CV = DPT < 4 ? DPT : 4;
+    // O goes to memory four columns at a time (short prompts 81.6 -> 80.0 us); with fewer rows it does not pay (three
+    // tokens of 15 requests: 47.8 us instead of 46.3)
+    static constexpr bool WIDE = R == 64;
     static constexpr int LDK = HDP + 4, LDP = R + 4;
     static constexpr int STAGE = SIMT_KT * (LDK + HDP);  // floats of a K and a V tile
     static constexpr size_t SMEM = sizeof(float) * (R * HDP + 2 * STAGE + SIMT_KT * LDP);
@@ -56,6 +59,20 @@ __device__ __forceinline__ void load16(const T *p, float (&f)[16 / sizeof(T)]) {
     const T *t = reinterpret_cast<const T *>(&r);
 #pragma unroll
     for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = to_f(t[i]);
+}
+
+// Four consecutive elements, aligned as such
+template <typename T>
+__device__ __forceinline__ void store4(T *p, float a, float b, float c, float d) {
+    struct alignas(4 * sizeof(T)) {
+        T t[4];
+    } x;
+    from_f(x.t[0], a);
+    from_f(x.t[1], b);
+    from_f(x.t[2], c);
+    from_f(x.t[3], d);
+    if constexpr (sizeof x == 16) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<uint4 *>(&x);
+    else *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(&x);
 }
 
 __device__ __forceinline__ void copy16(void *dst, const void *src, int bytes) {  // zeros past `bytes`
@@ -274,8 +291,14 @@ __global__ void __launch_bounds__(SimtCfg<HDP, R>::THREADS) attn_simt_kernel(con
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 4 * ty + i;
+                if constexpr (C::WIDE) {
 #pragma unroll
-                for (int d = 0; d < DPT; ++d) mine[r * HDP + col(d)] = o[i][d];
+                    for (int d = 0; d < DPT; d += 4)
+                        store4(mine + r * HDP + col(d), o[i][d], o[i][d + 1], o[i][d + 2], o[i][d + 3]);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < DPT; ++d) mine[r * HDP + col(d)] = o[i][d];
+                }
                 if (tx == 0) {
                     mine[R * HDP + r] = m[i];
                     mine[R * HDP + R + r] = l[i];
@@ -307,8 +330,19 @@ __global__ void __launch_bounds__(SimtCfg<HDP, R>::THREADS) attn_simt_kernel(con
                     const int r = 4 * ty + i;
                     pm[i] = __ldcg(p + R * HDP + r);
                     pl[i] = __ldcg(p + R * HDP + R + r);
+                    if constexpr (C::WIDE) {
 #pragma unroll
-                    for (int d = 0; d < DPT; ++d) po[i][d] = __ldcg(p + r * HDP + col(d));
+                        for (int d = 0; d < DPT; d += 4) {
+                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + r * HDP + col(d)));
+                            po[i][d] = x.x;
+                            po[i][d + 1] = x.y;
+                            po[i][d + 2] = x.z;
+                            po[i][d + 3] = x.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < DPT; ++d) po[i][d] = __ldcg(p + r * HDP + col(d));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -335,9 +369,16 @@ __global__ void __launch_bounds__(SimtCfg<HDP, R>::THREADS) attn_simt_kernel(con
             }
             const float inv = none ? 0.0f : __fdiv_rn(corr, total);
             T *out = reinterpret_cast<T *>(a.out) + (int64_t)(w.s.q0 + tok) * a.os[0] + (int64_t)h * a.os[1];
+            auto value = [&](int d) -> float { return none ? 0.0f : __fmul_rn(o[i][d], inv); };
+            if constexpr (C::WIDE) {
 #pragma unroll
-            for (int d = 0; d < DPT; ++d)
-                if (col(d) < a.D) from_f(out[col(d)], none ? 0.0f : __fmul_rn(o[i][d], inv));
+                for (int d = 0; d < DPT; d += 4)
+                    if (col(d) < a.D) store4(out + col(d), value(d), value(d + 1), value(d + 2), value(d + 3));
+            } else {
+#pragma unroll
+                for (int d = 0; d < DPT; ++d)
+                    if (col(d) < a.D) from_f(out[col(d)], value(d));
+            }
         }
     }
 }
