@@ -46,10 +46,10 @@
 // more than they save: unrolling the weights' loop by two took 16 prompts from
 // 338 to 393 us); an item costs about 6000 more.  At head size 128 the two S
 // buffers leave each row tile waiting for its products (2000 of 4300 cycles a
-// tile).  Measured: 16 prompts of 100-2048 tokens, 64 query over 8 KV heads of
-// 64, bf16: 309 us, 516 TFLOP/s; four of 1500-4000 with a window of 128: 145
-// us, 1.5 TB/s; one of 8191, 32 over 8 heads of 128, f16: 610 us, 900 TFLOP/s
-// (cuBLAS bf16 1669).
+// tile; S in halves of 64 keys or the row tiles in turn: no better).  Measured:
+// 16 prompts of 100-2048 tokens, 64 query over 8 KV heads of 64, bf16: 309 us,
+// 516 TFLOP/s; four of 1500-4000 with a window of 128: 145 us, 1.5 TB/s; one of
+// 8191, 32 over 8 heads of 128, f16: 605 us, 910 TFLOP/s (cuBLAS bf16 1669).
 #include <algorithm>
 #include <climits>
 
