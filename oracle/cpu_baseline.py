@@ -78,6 +78,7 @@ def measure(D=2880, H=64, KVH=8, hd=64, E=128, K=4, inter=2880, V=201088, gs=32,
                         rng.uniform(1e-3, 2e-3, D * (inter // gs)).astype(f32), rng.standard_normal(D).astype(f32) * 0.01))
     x = rng.standard_normal(D).astype(f32)
     out = np.zeros(D, f32)
+    heads = np.zeros(H * hd, f32)  # the attention's output before its projection
 
     def layer(layer_type):
         pos = ctx - 1
@@ -88,7 +89,7 @@ def measure(D=2880, H=64, KVH=8, hd=64, E=128, K=4, inter=2880, V=201088, gs=32,
                                 _p(x, fp), _p(out, fp), D, H, KVH, hd, 150000.0)
         else:
             q = O.matmul_q8(x, wq, sq, H * hd, D)[0]
-            O.lib().or_attention(_p(out, fp), _p(np.ascontiguousarray(q[: H * hd]), fp), _p(Kc, fp), _p(Vc, fp),
+            O.lib().or_attention(_p(heads, fp), _p(np.ascontiguousarray(q[: H * hd]), fp), _p(Kc, fp), _p(Vc, fp),
                                  _p(sinks, fp), H, KVH, hd, 0 if layer_type else pos - window + 1, pos)
         O.router_topk(x, router, None, K)
         acc = np.zeros(D, f32)
