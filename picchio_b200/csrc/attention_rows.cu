@@ -312,6 +312,7 @@ static __device__ __noinline__ void scale_o(uint32_t ot, int cols, float corr) {
 template <typename T>
 __device__ __noinline__ void scale_p(uint32_t st, int cols, float corr) {
     using E = Half16<T>;
+    tmem_st_wait();  // this thread's own stores of them: without the wait a load may come before them
 #pragma unroll 1
     for (int x = 0; x < cols; x += 16) {
         uint32_t ov[16];

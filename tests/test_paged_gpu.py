@@ -379,6 +379,30 @@ def test_scores_that_grow_late(dtype, window):
     close(out, want, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("group", [1, 2, 3])
+def test_scores_that_grow_within_the_first_tile(dtype, D, group):
+    """Of the first 128 keys one group of 32 outweighs the groups before it by
+    2^10, with the groups' weights written one after another: what is written
+    has to follow the new reference.  All rows that see the tile whole, and
+    those that see a part."""
+    torch = _torch()
+    n, H, KH = 420, 4, 2
+    g = gen(40 + group)
+    q, k, v = (torch.randn(n, h, D, generator=g, device="cuda") for h in (H, KH, KH))
+    k = k * 0.25
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    k[32 * group:, :, 0] = 10 * math.log(2) * math.sqrt(D) / 8
+    q, k, v = (x.to(_dt(dtype)) for x in (q, k, v))
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    for window in (0, 140):
+        out = handle().packed(q, k, v, cu, window=window)
+        want, bound = reference(q, k, v, 0, None, window, D ** -0.5, dtype)
+        close(out, want, bound)
+
+
 def test_same_inputs_same_bits():
     """Items split between blocks are joined in a fixed order."""
     torch = _torch()
