@@ -29,8 +29,10 @@
 // where all are seen, else that of its first tile), and later scores are not
 // searched for their maximum first: the sum of 32 weights shows when one has
 // grown past 2^14 (f16 weights, stored 2^7 up, end at 2^16), and then the tile
-// is gone through the careful way from there on: maximum, reference moved by a
-// power of two, O and what is written of the tile rescaled.  (Each item's first
+// is gone through the careful way from there on: maximum, reference moved to
+// it, O and what is written of the tile rescaled.  References are whole
+// numbers (of powers of two, the next above the maximum), so that two of them
+// near one another differ by exactly what the rescaling takes.  (Each item's first
 // tile searched whole: 16 prompts 341 us instead of 312.)
 //
 // A key that a row does not see has weight 0, but 0 x NaN is NaN: in tiles
@@ -63,6 +65,7 @@ namespace {
 constexpr int RW_R = 256, RW_KT = 128, RW_OV = 256, RW_MINK = 256, RW_THREADS = 384;
 constexpr float RW_GROW = 8.0f;       // log2 of the growth that moves the reference in the careful way
 constexpr float RW_LIMIT = 16384.0f;  // what 32 weights of a row may sum up to before it is taken
+constexpr float RW_FAR = 8388608.0f;  // references from here on (2^23): see far_scores
 
 template <int HD>
 struct RowsCfg {
@@ -305,6 +308,23 @@ static __device__ __noinline__ void scale_o(uint32_t ot, int cols, float corr) {
 #pragma unroll
         for (int y = 0; y < 16; ++y) ov[y] = __float_as_uint(__fmul_rn(__uint_as_float(ov[y]), corr));
         tmem_st16(ot + x, ov);
+    }
+    tmem_st_wait();
+}
+// A row's scores from column `from` on in the place of themselves, as powers of
+// two beside its reference.  Far from 0 score x c - reference, rounded once, is
+// off by as much as the reference is from the maximum's exact product (32
+// powers of two at f16's lowest value, any number at bf16's): here the product
+// is rounded first, as the reference was, and the maximum's own weight is 1.
+static __device__ __noinline__ void far_scores(uint32_t st, int from, float c, float ref) {
+#pragma unroll 1
+    for (int x = from; x < RW_KT; x += 16) {
+        uint32_t v[16];
+        tmem_ld16(st + x, v);
+        tmem_ld_wait16(v);
+#pragma unroll
+        for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[y]), c), ref));
+        tmem_st16(st + x, v);
     }
     tmem_st_wait();
 }
@@ -750,7 +770,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 const uint64_t c2 = f2_pack(c, c);
                 int xs = 0;  // the group from which on the careful way goes
                 bool grown = false;
-                if (all_see(0) && all_see(3) && (HD == 64 || __all_sync(0xffffffffu, mr != -INFINITY))) {
+                if (all_see(0) && all_see(3) && (HD == 64 || __all_sync(0xffffffffu, fabsf(mr) < RW_FAR))) {
                     // No look at the maximum first: the weights are taken against the reference as it is, and the
                     // sum of a group tells whether one has grown too large for it (or is no number).
                     tmem_ld32(st, sv);
@@ -759,11 +779,11 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                         tmem_ld_wait32(sv);
 #pragma unroll
                         for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
-                        if (mr == -INFINITY) mr = mx < INFINITY ? __fmul_rn(mx, c) : NAN;
+                        if (mr == -INFINITY) mr = mx < INFINITY ? ceilf(__fmul_rn(mx, c)) : NAN;
                     }
                     const float nmc = __fsub_rn(E::BIAS, mr);
                     const uint64_t nmc2 = f2_pack(nmc, nmc);
-                    if (HD == 128 || __all_sync(0xffffffffu, mr != -INFINITY))  // else none but -inf so far
+                    if (HD == 128 || __all_sync(0xffffffffu, fabsf(mr) < RW_FAR))  // else none but -inf so far, or far off
 #pragma unroll(HD == 128 ? 2 : 1)
                     for (; xs < 4; ++xs) {
                         uint64_t v[16], part[2] = {0, 0};
@@ -791,7 +811,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                 if (xs < 4) {
                     // the careful way, from group xs on: tiles that some row does not see whole; the maximum is searched
                     // for where a row has no reference yet, or its own has been outgrown
-                    bool search = grown || __any_sync(0xffffffffu, mr == -INFINITY);
+                    bool search = grown || !__all_sync(0xffffffffu, fabsf(mr) < RW_FAR);
                     do {
                         if (search) {
                             float mx = -INFINITY;
@@ -803,13 +823,15 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
 #pragma unroll
                                 for (int y = 0; y < 16; ++y) mx = max3(mx, __uint_as_float(sv[2 * y]), __uint_as_float(sv[2 * y + 1]));
                             }
-                            // move the reference of rows that have none, or whose maximum has grown
-                            const float top = __fmul_rn(mx, c), grow = ceilf(__fsub_rn(top, mr));
+                            // move the reference of rows that have none, or whose maximum has grown, to that maximum itself
+                            // (the old one plus the growth would be the maximum rounded to the old one's spacing: 64 after
+                            // scores of f16's lowest value)
+                            const float top = ceilf(__fmul_rn(mx, c)), grow = __fsub_rn(top, mr);  // exact where it is below 126
                             float corr = 1.0f;
                             if (mr == -INFINITY) {
                                 mr = top;
                             } else if (grow > (grown ? 0.0f : RW_GROW)) {
-                                mr = __fadd_rn(mr, grow);
+                                mr = top;
                                 corr = grow < 126.0f ? __int_as_float((127 - (int)grow) << 23) : 0.0f;
                             }
                             if (!(mx < INFINITY)) mr = NAN;  // an infinite or NaN score: so are the row's weights
@@ -825,8 +847,11 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                                 if (xs) scale_p<T>(st, 16 * xs, corr);
                             }
                         }
-                        const float nmc = mr == -INFINITY ? 0.0f : __fsub_rn(E::BIAS, mr);
-                        const uint64_t nmc2 = f2_pack(nmc, nmc);
+                        const float ref = mr == -INFINITY ? 0.0f : mr;
+                        const bool far = __any_sync(0xffffffffu, fabsf(ref) >= RW_FAR);  // then searched: all that is left follows
+                        if (far) far_scores(st, 32 * xs, c, ref);
+                        const float nmc = far ? E::BIAS : __fsub_rn(E::BIAS, ref), cc = far ? 1.0f : c;
+                        const uint64_t nmc2 = f2_pack(nmc, nmc), cc2 = f2_pack(cc, cc);
 #pragma unroll 1
                         for (; xs < 4; ++xs) {
                             uint32_t pk[16];
@@ -838,7 +863,7 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
                                 hide(sv, seen);
 #pragma unroll
                                 for (int y = 0; y < 16; ++y) {
-                                    const uint64_t p = f2_ex2(f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), c2, nmc2));
+                                    const uint64_t p = f2_ex2(f2_fma(f2_pack_bits(sv[2 * y], sv[2 * y + 1]), cc2, nmc2));
                                     part[y & 1] = f2_add(part[y & 1], p);
                                     pk[y] = E::pack(f2_lo(p), f2_hi(p));
                                 }

@@ -403,6 +403,37 @@ def test_scores_that_grow_within_the_first_tile(dtype, D, group):
         close(out, want, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("hidden", [32, 128, 200])
+@pytest.mark.parametrize("off", [0, 30, -29, 150, -150])
+def test_lowest_values_first(dtype, D, hidden, off):
+    """A request's first keys have f16's lowest value as their score's factor (the
+    usual mask): rows that see others give those the weights they have alone,
+    wherever their scores lie (2^off), and the first rows, which see none
+    other, the mean."""
+    torch = _torch()
+    reqs = [(700, 300), (400, 3), (520, 520)]
+    q, kp, vp, table, cu, kv = make_paged(reqs, 16, 4, 2, D, dtype, 51)
+    q[..., 0], q[..., 1] = 65504.0, 8.0
+    for b, (total, _) in enumerate(reqs):
+        pos = torch.arange(total, device="cuda")
+        at = table[b, pos // 16].long(), pos % 16
+        kk = kp[at]
+        kk[..., 0] = 0.0
+        kk[..., 1] = off * math.log(2) * math.sqrt(D) / 8
+        kk[:hidden] = 0.0
+        kk[:hidden, :, 0] = -65504.0
+        kp[at] = kk
+    for window in (0, 250):
+        out = handle().paged(q, kp, vp, table, cu, kv, window=window)
+        for b, (total, new) in enumerate(reqs):
+            r = slice(int(cu[b]), int(cu[b + 1]))
+            want, bound = reference(q[r], gathered(kp, table, b, total), gathered(vp, table, b, total), total - new, None,
+                                    window, D ** -0.5, dtype)
+            close(out[r], want, bound)
+
+
 def test_same_inputs_same_bits():
     """Items split between blocks are joined in a fixed order."""
     torch = _torch()
