@@ -249,6 +249,11 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
 #pragma unroll
                     for (int n = 0; n < NR; ++n) mma16<T>(sc4[i][n], f, qf[k][n][0], qf[k][n][1]);
                 }
+                // in powers of two, rounded here: maximum, weights and rescaling all go by the same numbers
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) sc4[i][n][x] = __fmul_rn(sc4[i][n][x], c);
             }
             const bool masked = k0 + KT - 1 > g.pmin || (a.window > 0 && k0 < g.pmax - a.window + 1);
             if (masked) {
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
             uint32_t pf[KT / 16][NR][2];
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-                float corr[2], nmc[2];
+                float corr[2], ms[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     float top = -INFINITY;
@@ -322,9 +327,9 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float mn = fmaxf(m[n][x], top), mc = mn == -INFINITY ? 0.0f : __fmul_rn(mn, c);
-                    corr[x] = ex2(__fmaf_rn(m[n][x], c, -mc));
-                    nmc[x] = __fsub_rn(E::BIAS, mc);
+                    const float mn = fmaxf(m[n][x], top);
+                    ms[x] = mn == -INFINITY ? 0.0f : mn;
+                    corr[x] = ex2(__fsub_rn(m[n][x], ms[x]));  // 1 while the maximum stands
                     m[n][x] = mn;
                     l[n][x] = __fmul_rn(l[n][x], corr[x]);
                 }
@@ -332,8 +337,8 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                 for (int i = 0; i < KT / 16; ++i)
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {  // keys g8, g8 + 8
-                        const float p0 = ex2(__fmaf_rn(sc4[i][n][2 * y], c, nmc[0]));
-                        const float p1 = ex2(__fmaf_rn(sc4[i][n][2 * y + 1], c, nmc[1]));
+                        const float p0 = ex2(__fadd_rn(__fsub_rn(sc4[i][n][2 * y], ms[0]), E::BIAS));
+                        const float p1 = ex2(__fadd_rn(__fsub_rn(sc4[i][n][2 * y + 1], ms[1]), E::BIAS));
                         l[n][0] = __fadd_rn(l[n][0], p0);
                         l[n][1] = __fadd_rn(l[n][1], p1);
                         pf[i][n][y] = turn8(E::pack(p0, p1));
@@ -382,7 +387,7 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                 ll = __fadd_rn(ll, __shfl_xor_sync(0xffffffffu, ll, 8));
                 ll = __fadd_rn(ll, __shfl_xor_sync(0xffffffffu, ll, 16));
                 if (g8 == 0) {
-                    wm[warp][row] = m[n][x] == -INFINITY ? m[n][x] : __fmul_rn(m[n][x], c);  // in powers of two
+                    wm[warp][row] = m[n][x];
                     wl[warp][row] = ll;
                 }
             }

@@ -434,6 +434,49 @@ def test_lowest_values_first(dtype, D, hidden, off):
             close(out[r], want, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 3, 130])
+def test_only_lowest_values(dtype, D, new):
+    """Every key has the type's lowest value as its score's factor: the mean of
+    V, with few rows and many.  The scores are alike, so only weights of 1, their
+    sums and the result are rounded."""
+    torch = _torch()
+    reqs = [(new, new), (300, new)]
+    q, kp, vp, table, cu, kv = make_paged(reqs, 16, 8, 4, D, dtype, 55, garbage=False)
+    q[..., 0] = 65504.0 if dtype == "f16" else 1.0
+    kp.zero_()
+    kp[..., 0] = torch.finfo(_dt(dtype)).min
+    out = handle().paged(q, kp, vp, table, cu, kv)
+    for b, (total, n) in enumerate(reqs):
+        r = slice(int(cu[b]), int(cu[b + 1]))
+        k = torch.zeros(total, 4, D, device="cuda")
+        want, bound = reference(q[r] * 0, k, gathered(vp, table, b, total), total - n, None, 0, D ** -0.5, dtype)
+        close(out[r], want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_contexts_weigh_old_and_new_keys_alike(dtype):
+    """One early key against 131,071 later ones of the same total weight, in
+    hundreds of tiles a warp that all leave the maximum as it is: a factor
+    beside 1 at each of them would add up (5e-6 a tile to 1e-3)."""
+    torch = _torch()
+    B, L, D, G, page = 296, 1 << 17, 8, 4, 64
+    k = torch.zeros(L // page, page, 1, D, device="cuda")
+    v = torch.full_like(k, -1.0)
+    k[..., 0], k[..., 1] = 100.0, -10.0
+    k[0, 0, :, 1], v[0, 0] = 0.0, 1.0
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda").expand(B, -1).contiguous()
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    kv = torch.full((B,), L, dtype=torch.int32, device="cuda")
+    q, k, v = (x.to(_dt(dtype)) for x in (torch.ones(B, G, D, device="cuda"), k, v))
+    for scale in (1.171, 1.1755, 1.18, 1.1843):
+        out = handle().paged(q, k, v, table, cu, kv, scale=scale)
+        handle().check()
+        want, bound = reference(q[:1], k.flatten(0, 1), v.flatten(0, 1), L - 1, None, 0, scale, dtype)
+        close(out, want.expand(out.shape), bound.expand(out.shape))
+
+
 def test_same_inputs_same_bits():
     """Items split between blocks are joined in a fixed order."""
     torch = _torch()
