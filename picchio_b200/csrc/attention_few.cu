@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                     for (int x = 0; x < 4; ++x) sc4[i][n][x] = __fmul_rn(sc4[i][n][x], c);
             }
             const bool masked = k0 + KT - 1 > g.pmin || (a.window > 0 && k0 < g.pmax - a.window + 1);
+            bool odd = false;  // non-finite V that only some rows see
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < KT / 16; ++i)
@@ -284,36 +285,7 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                     for (int y = 0; y < 4; ++y) bad |= (e[y] & E::EXP) == E::EXP || (e[y] >> 16 & E::EXP) == E::EXP;
                 }
                 __syncwarp();
-                if (__any_sync(0xffffffffu, bad)) {
-#pragma unroll 1
-                    for (int r = 0; r < KT; ++r) {
-                        const int key = k0 + r;
-                        if (key < g.kb || key >= g.ke) continue;
-#pragma unroll
-                        for (int d = 0; d < HD / 16; ++d)
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                const int c0 = d * 16 + g8 + 8 * (x >> 1), ch = c0 >> 3;
-                                const float f = E::up(*reinterpret_cast<const unsigned short *>(
-                                    v + (ch >> 3) * C::PANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4) + (c0 & 7) * 2));
-#pragma unroll
-                                for (int n = 0; n < NR; ++n) {
-                                    const int p = pos[n][x & 1];
-                                    if (!isfinite(f) && key <= p && !(a.window > 0 && key <= p - a.window))
-                                        o[d][n][x] = __fadd_rn(o[d][n][x], f);
-                                }
-                            }
-                    }
-                    __syncwarp();
-                    for (int i = lane; i < KT * C::PANELS * 32; i += 32) {
-                        uint32_t *q = reinterpret_cast<uint32_t *>(v) + i;
-                        uint32_t x = *q;
-                        if ((x & E::EXP) == E::EXP) x &= 0xFFFF0000u;
-                        if ((x >> 16 & E::EXP) == E::EXP) x &= 0x0000FFFFu;
-                        *q = x;
-                    }
-                    __syncwarp();
-                }
+                odd = __any_sync(0xffffffffu, bad);
             }
             uint32_t pf[KT / 16][NR][2];
 #pragma unroll
@@ -348,6 +320,37 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                     for (int d = 0; d < HD / 16; ++d)
 #pragma unroll
                         for (int x = 0; x < 4; ++x) o[d][n][x] = __fmul_rn(o[d][n][x], corr[x & 1]);
+            }
+            if (odd) {  // after the rescaling, whose first factor is 0
+                uint8_t *v = wring + (s * 2 + 1) * C::TILE;
+#pragma unroll 1
+                for (int r = 0; r < KT; ++r) {
+                    const int key = k0 + r;
+                    if (key < g.kb || key >= g.ke) continue;
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int c0 = d * 16 + g8 + 8 * (x >> 1), ch = c0 >> 3;
+                            const float f = E::up(*reinterpret_cast<const unsigned short *>(
+                                v + (ch >> 3) * C::PANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4) + (c0 & 7) * 2));
+#pragma unroll
+                            for (int n = 0; n < NR; ++n) {
+                                const int p = pos[n][x & 1];
+                                if (!isfinite(f) && key <= p && !(a.window > 0 && key <= p - a.window))
+                                    o[d][n][x] = __fadd_rn(o[d][n][x], f);
+                            }
+                        }
+                }
+                __syncwarp();
+                for (int i = lane; i < KT * C::PANELS * 32; i += 32) {
+                    uint32_t *q = reinterpret_cast<uint32_t *>(v) + i;
+                    uint32_t x = *q;
+                    if ((x & E::EXP) == E::EXP) x &= 0xFFFF0000u;
+                    if ((x >> 16 & E::EXP) == E::EXP) x &= 0x0000FFFFu;
+                    *q = x;
+                }
+                __syncwarp();
             }
             // O^T += V^T P^T
 #pragma unroll

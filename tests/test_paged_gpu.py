@@ -328,6 +328,28 @@ def test_unseen_keys_have_no_part(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [2, 3, 6])
+def test_unseen_keys_have_no_part_with_few_rows(dtype, D, new):
+    """The same through the pages, a few new tokens a request: infinities and
+    NaN in the last positions, which the first of the new rows do not see."""
+    reqs = [(300, new), (40, new), (900, new)]
+    q, kp, vp, table, cu, kv = make_paged(reqs, 16, 8, 4, D, dtype, 61)
+    for b, (total, _) in enumerate(reqs):
+        for back, head, x, val in ((1, 0, 3, "inf"), (new, 1, 5, "-inf"), (new - 1, 2, 7, "nan"), (1, 3, slice(None), "inf"),
+                                   (20, 3, 2, "-inf")):
+            p = total - back
+            vp[int(table[b, p // 16]), p % 16, head, x] = float(val)
+    for window in (0, 7):
+        out = handle().paged(q, kp, vp, table, cu, kv, window=window)
+        for b, (total, n) in enumerate(reqs):
+            r = slice(int(cu[b]), int(cu[b + 1]))
+            want, bound = reference(q[r], gathered(kp, table, b, total), gathered(vp, table, b, total), total - n, None,
+                                    window, D ** -0.5, dtype)
+            close(out[r], want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_large_scores(dtype):
     """Scores far apart: the running maximum moves, weights underflow."""
     torch = _torch()
