@@ -375,8 +375,10 @@ pc_status pc_kv_store(int device, const pc_kv_pages *kv, const void *k_dev, cons
  *   s_j = scale * q . k_j, m the largest s_j or sink_h
  * (without sinks, no sink term).  Keys a row does not see have no part in
  * it, whatever their K and V hold (stale pages, NaN).  A row that sees no key
- * gives zeros.  Sums and softmax statistics are fp32; for 16-bit types the
- * softmax weights are rounded to that type before they meet V. */
+ * gives zeros.  Sums and softmax statistics are fp32.  For 16-bit types the
+ * softmax weights meet V as two numbers of that type, together good to 2^-16;
+ * those of requests with many rows (more than 16 and more than n_heads /
+ * n_kv_heads over pages; all in pc_attn_packed) as one, rounded. */
 typedef struct {
     const void *q_dev;     /* [n_rows][n_heads][head_dim] */
     int64_t q_stride[2];   /* elements: row, head */

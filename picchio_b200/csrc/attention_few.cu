@@ -9,7 +9,11 @@
 // own running maximum, sum and O in registers.  The products are mma.sync
 // m16n8k16 with the few rows as the N side: S^T = K Q^T (16 keys x 8 rows) and
 // O^T += V^T P^T (16 head columns x 8 rows), so eight rows leave nothing of a
-// product unused; P^T turns from accumulator to operand by movmatrix.  (With
+// product unused; P^T turns from accumulator to operand by movmatrix.  P is
+// rounded to the type, and what the rounding left has a product of its own: the
+// tensor pipe has room, and the error of bf16 outputs is that of their own
+// rounding (decode of 64 requests 1.97e-3 -> 1.66e-3 from the exact result; 109.5
+// -> 110.0 us, head size 128 184.4 -> 186.0).  (With
 // the rows as the M side, half of the products and of the exponentials were of
 // rows that did not exist: head size 128 211 us where it is 184 now, one token
 // 16 us where it is 14.)  The legacy products are far below their rate while
@@ -24,8 +28,8 @@
 // workspace.
 //
 // Measured: one token each of 64 requests of 500-8000 positions, 64 query over
-// 8 KV heads of 64, bf16, pages of 16: 109 us, 5.4 TB/s (83 % of the measured
-// copy); 32 over 8 heads of 128, f16, pages of 32: 184 us, 6.5 TB/s (99 %).
+// 8 KV heads of 64, bf16, pages of 16: 110 us, 5.4 TB/s (83 % of the measured
+// copy); 32 over 8 heads of 128, f16, pages of 32: 186 us, 6.4 TB/s (98 %).
 // 64-wide heads read 128 bytes of each 1 KB row; with pages laid out heads
 // first they are 6 % faster.  One token over 4096 positions takes 14 us: 2.5 us
 // to find the shares, about 2 until the first tile is there, the rest its work,
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                 __syncwarp();
                 odd = __any_sync(0xffffffffu, bad);
             }
-            uint32_t pf[KT / 16][NR][2];
+            uint32_t pf[KT / 16][NR][2], pr[KT / 16][NR][2];  // weights in the type, and what that rounding left
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
                 float corr[2], ms[2];
@@ -313,7 +317,9 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                         const float p1 = ex2(__fadd_rn(__fsub_rn(sc4[i][n][2 * y + 1], ms[1]), E::BIAS));
                         l[n][0] = __fadd_rn(l[n][0], p0);
                         l[n][1] = __fadd_rn(l[n][1], p1);
-                        pf[i][n][y] = turn8(E::pack(p0, p1));
+                        const uint32_t h = E::pack(p0, p1);
+                        pf[i][n][y] = turn8(h);
+                        pr[i][n][y] = turn8(E::pack(__fsub_rn(p0, E::up(h & 0xFFFFu)), __fsub_rn(p1, E::up(h >> 16))));
                     }
                 if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f))
 #pragma unroll
@@ -352,17 +358,32 @@ __global__ void __launch_bounds__(FW_THREADS, FW_PER_SM)
                 }
                 __syncwarp();
             }
-            // O^T += V^T P^T
+            // O^T += V^T P^T; what the weights' rounding left apart, so that a V that is infinite does not meet it (0 or
+            // below: inf would become NaN)
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d)
+            for (int d = 0; d < HD / 16; ++d) {
+                float rest[NR][4];
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) rest[n][x] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < KT / 16; ++i) {
                     uint32_t f[4];
                     const int j = lane >> 3, row = 16 * i + (lane & 7) + 8 * (j >> 1), ch = 2 * d + (j & 1);
                     ldsm4_t(f, vt + (ch >> 3) * C::PANEL + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) mma16<T>(o[d][n], f, pf[i][n][0], pf[i][n][1]);
+                    for (int n = 0; n < NR; ++n) {
+                        mma16<T>(o[d][n], f, pf[i][n][0], pf[i][n][1]);
+                        mma16<T>(rest[n], f, pr[i][n][0], pr[i][n][1]);
+                    }
                 }
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        o[d][n][x] = isfinite(o[d][n][x]) ? __fadd_rn(o[d][n][x], rest[n][x]) : o[d][n][x];
+            }
             if (masked) fence_async_smem();  // V rows written here, and by TMA next
             __syncwarp();
             fetch();

@@ -499,6 +499,25 @@ def test_long_contexts_weigh_old_and_new_keys_alike(dtype):
         close(out, want.expand(out.shape), bound.expand(out.shape))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 3])
+def test_few_rows_lose_nothing_in_the_weights(dtype, D, new):
+    """With few rows the weights keep what their rounding leaves: of the bound
+    the type's part falls on the result alone (u |out|), the rest (2^-14 A) on
+    the weights' second rounding (2^-16 A bf16), sums and exponentials."""
+    reqs = [(5000, new), (300, new), (17, new)]
+    q, kp, vp, table, cu, kv = make_paged(reqs, 16, 16, 4, D, dtype, 71)
+    out = handle().paged(q, kp, vp, table, cu, kv)
+    for b, (total, n) in enumerate(reqs):
+        r = slice(int(cu[b]), int(cu[b + 1]))
+        k, v = gathered(kp, table, b, total), gathered(vp, table, b, total)
+        want, _ = reference(q[r], k, v, total - n, None, 0, D ** -0.5, dtype)
+        A, _ = reference(q[r], k, v.abs(), total - n, None, 0, D ** -0.5, dtype)
+        tiny = 2.0 ** -25 if dtype == "f16" else 0.0
+        close(out[r], want, (U[dtype] * want.abs() + 2.0 ** -14 * A + tiny) * 1.02 + 1e-30)
+
+
 def test_same_inputs_same_bits():
     """Items split between blocks are joined in a fixed order."""
     torch = _torch()
