@@ -48,6 +48,24 @@ __device__ __forceinline__ SeqGeo seq_geo(const AttnOp &a, int b) {
     return s;
 }
 
+// Whether a kernel that takes min_q <= rows <= max_q takes request b.
+__device__ __forceinline__ bool takes(const int *cu, int b, int T, int G, int min_q, int max_q) {
+    const int lo = min(max(__ldcg(cu + b), 0), T), hi = min(max(__ldcg(cu + b + 1), 0), T);
+    const int rows = max(hi - lo, 0) * G;
+    return rows >= min_q && rows <= max_q;
+}
+
+// The next request after b that a kernel takes, or one past `last`; a warp
+// calls it, so that slots without a request cost little.
+__device__ __forceinline__ int next_request(const int *cu, int b, int last, int T, int G, int min_q, int max_q) {
+    for (int b0 = b + 1; b0 <= last; b0 += 32) {
+        const int mine = b0 + (int)(threadIdx.x & 31);
+        const unsigned m = __ballot_sync(0xffffffffu, mine <= last && takes(cu, mine, T, G, min_q, max_q));
+        if (m) return b0 + __ffs(m) - 1;
+    }
+    return last + 1;
+}
+
 // Rows [r0, r1) of the request's tokens x group, keys [kb, ke), tiles of KT
 // from tile t0 on (at least one, so that rows without keys are written).
 struct ItemGeo {
@@ -232,8 +250,9 @@ struct PlanWalk {
     __device__ __forceinline__ bool load(bool request = true) {
         if (b >= a.B) return false;
         if (request) s = seq_geo<R>(a, b);
-        while (s.n_items == 0) {
-            if (++b >= a.B) return false;
+        if (s.n_items == 0) {
+            b = next_request(a.cu, b, min(sh.e.b, a.B - 1), a.T, a.G, a.min_q, a.max_q);
+            if (b >= a.B) return false;
             s = seq_geo<R>(a, b);
         }
         const bool at_end = b == sh.e.b && kvh == sh.e.kvh && item == sh.e.item;

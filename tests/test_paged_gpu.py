@@ -280,6 +280,40 @@ def test_packed(dtype, lens, H, KH, D, window, sinks):
         close(out[r], want, bound)
 
 
+def best_time(f):
+    """The least of 12 times of 8 calls."""
+    torch = _torch()
+    times = []
+    for _ in range(12):
+        e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        e[0].record()
+        for _ in range(8):
+            f()
+        e[1].record()
+        e[1].synchronize()
+        times.append(e[0].elapsed_time(e[1]))
+    return min(times)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_empty_prompts_cost_little(dtype):
+    """A thread block's way over slots without a prompt is short (one by one
+    the 511 behind the last prompt took as long as the prompt)."""
+    torch = _torch()
+    n = 1000
+    q, k, v = (torch.randn(n, h, 64, generator=gen(5), device="cuda").to(_dt(dtype)) for h in (64, 8, 8))
+    alone = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    among = torch.tensor([0] * 513 + [n] * 512, dtype=torch.int32, device="cuda")
+    gaps = torch.tensor([0] * 300 + [n // 3] * 300 + [n // 2] * 31 + [n] * 394, dtype=torch.int32, device="cuda")
+    assert torch.equal(handle().packed(q, k, v, among), handle().packed(q, k, v, alone))
+    out = handle().packed(q, k, v, gaps)
+    for a, b in ((0, n // 3), (n // 3, n // 2), (n // 2, n)):
+        want, bound = reference(q[a:b], k[a:b], v[a:b], 0, None, 0, 0.125, dtype)
+        close(out[a:b], want, bound)
+    one, many = best_time(lambda: handle().packed(q, k, v, alone)), best_time(lambda: handle().packed(q, k, v, among))
+    assert many < 1.6 * one, (many, one)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_heads_that_are_one(dtype):
     """K and V expanded over heads (strides of zero): no tensor map has them."""
