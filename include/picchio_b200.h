@@ -377,8 +377,9 @@ pc_status pc_kv_store(int device, const pc_kv_pages *kv, const void *k_dev, cons
  * it, whatever their K and V hold (stale pages, NaN).  A row that sees no key
  * gives zeros.  Sums and softmax statistics are fp32.  For 16-bit types the
  * softmax weights meet V as two numbers of that type, together good to 2^-16;
- * those of requests with many rows (more than 16 and more than n_heads /
- * n_kv_heads over pages; all in pc_attn_packed) as one, rounded. */
+ * those of many rows (pc_attn_packed; over pages beyond 16 rows x query heads
+ * of a KV head, unless one token has as many or the batch no more than 128) as
+ * one, rounded. */
 typedef struct {
     const void *q_dev;     /* [n_rows][n_heads][head_dim] */
     int64_t q_stride[2];   /* elements: row, head */

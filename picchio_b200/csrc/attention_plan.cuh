@@ -55,6 +55,17 @@ __device__ __forceinline__ bool takes(const int *cu, int b, int T, int G, int mi
     return rows >= min_q && rows <= max_q;
 }
 
+// Whether a launch beside another of the same call (min_q > 1) finds no request
+// to take; every thread of the block calls it, before pdl_wait.  The launch
+// before it lets this one start only after its own wait, so `cu` is written by
+// then; the block must wait as well before it ends, since what comes next waits
+// for this launch alone.
+__device__ __forceinline__ bool nothing_to_take(const int *cu, int B, int T, int G, int min_q, int max_q) {
+    bool any = false;
+    for (int b = threadIdx.x; b < B; b += blockDim.x) any |= takes(cu, b, T, G, min_q, max_q);
+    return !__syncthreads_or(any);
+}
+
 // The next request after b that a kernel takes, or one past `last`; a warp
 // calls it, so that slots without a request cost little.
 __device__ __forceinline__ int next_request(const int *cu, int b, int last, int T, int G, int min_q, int max_q) {

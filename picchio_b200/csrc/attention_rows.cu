@@ -372,6 +372,11 @@ __global__ void __launch_bounds__(RW_THREADS, 1)
     __shared__ volatile int odd[4];  // [i % 4] = i + 1: non-finite V in a masked tile of the block's item i
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    if (a.min_q > 1 && nothing_to_take(a.cu, a.B, a.T, a.G, a.min_q, a.max_q)) {
+        pdl_trigger();
+        pdl_wait();
+        return;
+    }
     if (tid == 0) {
         for (int t = 0; t < 4; ++t) {
             mbar_init(&bar.q_full[t], 1);

@@ -101,6 +101,11 @@ __global__ void __launch_bounds__(SimtCfg<HDP, R>::THREADS) attn_simt_kernel(con
     float *Qs = simt_smem, *ring = Qs + R * HDP, *Pt = ring + 2 * C::STAGE;
     __shared__ PlanScratch<C::THREADS> sc;
     __shared__ int lastf;
+    if (a.min_q > 1 && nothing_to_take(a.cu, a.B, a.T, a.G, a.min_q, a.max_q)) {
+        pdl_trigger();
+        pdl_wait();
+        return;
+    }
     pdl_wait();
     pdl_trigger();
     plan_share<R, KT, SIMT_OV, 2 * KT, C::THREADS>(a, blockIdx.x, gridDim.x, sc);
@@ -401,13 +406,30 @@ cudaError_t simt_run(const AttnOp &a, int nsm, cudaStream_t st) {
                     SimtCfg<HDP, R>::SMEM, st, a);
 }
 
-// The least rows an item that hold the batch's rows a request (and KV head)
+// The least rows an item that hold the batch's rows a request (and KV head) on
+// average: at fewer rows the products of rows that do not exist cost most (64
+// single tokens over 1000 positions, 8 query heads a group: 16 rows 156 us, 32
+// 205, 64 288).  Requests of more than 32 rows have a launch of their own with 64
+// (the average says nothing about the longest: 1024 tokens of one among 511 slots
+// without a request 620 us with 16 rows, 322 with this), unless there are so few
+// rows in all that one request of them all can do without (over 4096 positions,
+// 64- and 128-wide heads: 64 rows by 16 48 and 104 us, by 64 49 and 63; 512 rows
+// by 32 200 and 477, by 64 152 and 324).  The launch costs 1 to 3 us where it
+// finds nothing to do (three tokens of 15 requests 47 -> 50).
+constexpr int SIMT_FEW = 32, SIMT_ALONE16 = 64, SIMT_ALONE32 = 512;
+
 template <typename T, int HDP>
 cudaError_t simt_rows(const AttnOp &a, int nsm, cudaStream_t st) {
     const int64_t rows = (int64_t)a.T * a.G;
-    if (rows <= (int64_t)16 * a.B) return simt_run<T, HDP, 16>(a, nsm, st);
-    if (rows <= (int64_t)32 * a.B) return simt_run<T, HDP, 32>(a, nsm, st);
-    return simt_run<T, HDP, 64>(a, nsm, st);
+    if (rows > (int64_t)SIMT_FEW * a.B) return simt_run<T, HDP, 64>(a, nsm, st);
+    const bool r16 = rows <= (int64_t)16 * a.B, alone = rows <= (r16 ? SIMT_ALONE16 : SIMT_ALONE32);
+    AttnOp few = a, many = a;
+    if (!alone) {
+        few.max_q = std::min(a.max_q, SIMT_FEW);
+        many.min_q = std::max(a.min_q, SIMT_FEW + 1);
+    }
+    const cudaError_t e = r16 ? simt_run<T, HDP, 16>(few, nsm, st) : simt_run<T, HDP, 32>(few, nsm, st);
+    return e == cudaSuccess && !alone ? simt_run<T, HDP, 64>(many, nsm, st) : e;
 }
 
 template <typename T>

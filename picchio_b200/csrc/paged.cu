@@ -112,10 +112,25 @@ AttnOp op_of(const pc_attn *a, const pc_attn_call *c) {
 // f16 and bf16 have two kernels: one for few rows of a request and KV head
 // (tokens x query heads of the group), bound by reading K and V, and one for
 // many, bound by the products.  Which a request takes goes by its own rows,
-// read on the device; where the batch has no more rows than the first takes
-// of each request, the second is not launched (a request of more rows then
-// takes the first in several passes), and over whole prompts the first is not.
-constexpr int FEW_ROWS = 16;
+// read on the device; over whole prompts only the second is launched.
+//
+// Up to FEW_ROWS rows, and up to FEW_GROUP where a token alone has that many,
+// take the first.  It reads the keys once per 16 rows, the second once per 256.
+// 64 requests over 2000 positions, first and second, us: 64-wide heads, 8 a
+// group, 16 rows 62 and 127, 32 rows 106 and 127, 48 rows 149 and 127; 128-wide,
+// 4 a group, 16 rows 101 and 175, 32 rows 181 and 176; single tokens of 64 heads
+// a group 33 and 37, of 128 heads 51 and 37 (128-wide 83 and 53).
+//
+// The second is launched unless the whole batch has so few rows that one
+// request of them all does not need it: the host does not know how the rows are
+// shared out (slots without a request have none), and the average says
+// nothing about the longest.  The launch costs 1 to 5 us where it finds nothing to
+// do (64 single tokens over 500-8000 positions 111 -> 115, 16 over 2000 20 ->
+// 21.5); without it 512 rows of one request over 32,768 positions take 263 us
+// instead of 79, 1024 tokens of one among 511 slots without a request 169 instead
+// of 45.  At 128 rows of one request: over 4096 positions 25 us without, 30 with
+// it, over 32,768 79 and 65.
+constexpr int FEW_ROWS = 16, FEW_GROUP = 64, FEW_ALONE = 128;
 
 pc_status run_attention(pc_attn *a, const AttnOp &o, int dtype, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
@@ -127,9 +142,9 @@ pc_status run_attention(pc_attn *a, const AttnOp &o, int dtype, cudaStream_t st)
             }
         } else {
             AttnOp few = o, many = o;
-            const bool all_few = (int64_t)o.T * o.G <= (int64_t)std::max(o.G, FEW_ROWS) * o.B;
+            const bool all_few = (int64_t)o.T * o.G <= FEW_ALONE;
             if (!all_few) {
-                few.max_q = std::max(o.G, FEW_ROWS);
+                few.max_q = o.G <= FEW_GROUP ? std::max(o.G, FEW_ROWS) : FEW_ROWS;
                 many.min_q = few.max_q + 1;
             }
             if (launch_attn_few(few, dtype, a->nsm, st, e)) {

@@ -315,6 +315,28 @@ def test_empty_prompts_cost_little(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KH,D", [(8, 2, 64), (8, 1, 64), (8, 2, 128), (40, 1, 64), (96, 1, 8)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_paged_one_long_among_many(dtype, H, KH, D, window):
+    """One chunk among slots without a request, and beside single tokens: the
+    longest request has far more rows than the average."""
+    check_paged([(0, 0)] * 20 + [(500, 170)] + [(0, 0)] * 40, 16, H, KH, D, dtype, True, window)
+    check_paged([(50, 1)] * 9 + [(300, 90)] + [(0, 0)] * 40 + [(20, 1)] * 9, 16, H, KH, D, dtype, False, window)
+    check_paged([(300, 1), (0, 0), (260, 6), (0, 0)], 16, H, KH, D, dtype, False, window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_idle_slots_cost_little(dtype):
+    """A prompt among slots without a request runs as it does alone (a choice of
+    the kernel by the average rows a request made it 4 times as long in 16 bits,
+    twice in fp32)."""
+    alone, among = (make_paged(r, 16, 64, 8, 64, dtype, 3, garbage=False)
+                    for r in ([(1500, 1500)], [(0, 0)] * 512 + [(1500, 1500)] + [(0, 0)] * 511))
+    one, many = best_time(lambda: handle().paged(*alone)), best_time(lambda: handle().paged(*among))
+    assert many < 1.6 * one, (many, one)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_heads_that_are_one(dtype):
     """K and V expanded over heads (strides of zero): no tensor map has them."""
     torch = _torch()
