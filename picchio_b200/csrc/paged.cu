@@ -12,7 +12,7 @@
 #include "paged.h"
 
 struct pc_attn {
-    int dev = 0, nsm = 148, max_smem = 0;
+    int dev = 0, nsm = 148;
     float *part = nullptr;
     unsigned *ticket = nullptr;
     int *err = nullptr;
@@ -212,7 +212,6 @@ pc_status pc_attn_create(int device, pc_attn **out) {
         return s;
     };
     cudaError_t e = cudaDeviceGetAttribute(&a->nsm, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&a->max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
     if (e == cudaSuccess) e = attn_simt_configure();
     if (e == cudaSuccess) e = attn_rows_configure();
     if (e == cudaSuccess) e = attn_few_configure();
