@@ -228,6 +228,9 @@ class Attention:
         request b; ``k_pages``, ``v_pages`` [pages, page_size, kv_heads,
         head_dim]; ``page_table`` [B, max_pages], ``cu_new`` [B + 1],
         ``kv_len`` [B] int32: positions in the cache, the new rows' included.
+        Rows from ``cu_new[-1]`` on (padding of the step's tensors) are not
+        written: in a tensor made by the call they hold anything, NaN too;
+        give a zeroed ``out`` where they go on into other operators.
         """
         dev = self.device
         p, heads, _ = _pages(k_pages, v_pages, dev)
@@ -242,7 +245,8 @@ class Attention:
     def packed(self, q, k, v, cu_new, *, sinks=None, window: int = 0, scale=None, out=None, stream=None):
         """Attention over whole prompts packed into one tensor (pc_attn_packed):
         ``q`` [rows, heads, head_dim], ``k``, ``v`` [rows, kv_heads, head_dim],
-        rows ``cu_new[b] : cu_new[b + 1]`` of prompt b."""
+        rows ``cu_new[b] : cu_new[b + 1]`` of prompt b; as with :meth:`paged`,
+        rows from ``cu_new[-1]`` on are not written."""
         dev = self.device
         shape, ks = _heads3(k, "k", dev)
         vshape, vs = _heads3(v, "v", dev)

@@ -337,6 +337,24 @@ def test_idle_slots_cost_little(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_padding_rows_are_left_alone(dtype):
+    """Rows past the last request's are not written, whatever q holds there."""
+    torch = _torch()
+    for new in (1, 60):
+        q, kp, vp, table, cu, kv = make_paged([(70, new), (200, new)], 16, 8, 2, 64, dtype, 6)
+        rows = torch.full((2 * new + 150, 8, 64), float("nan"), dtype=q.dtype, device="cuda")
+        rows[:2 * new] = q
+        out = torch.full_like(rows, 7.0)
+        handle().paged(rows, kp, vp, table, cu, kv, out=out)
+        assert torch.isfinite(out[:2 * new].float()).all() and (out[2 * new:] == 7.0).all()
+        out.fill_(7.0)
+        k, v = (torch.randn(2 * new + 150, 2, 64, device="cuda").to(q.dtype) for _ in range(2))
+        k[2 * new:] = v[2 * new:] = float("nan")
+        handle().packed(rows, k, v, cu, out=out)
+        assert torch.isfinite(out[:2 * new].float()).all() and (out[2 * new:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_heads_that_are_one(dtype):
     """K and V expanded over heads (strides of zero): no tensor map has them."""
     torch = _torch()
