@@ -190,13 +190,46 @@ def kv_store(k_pages, v_pages, k, v, slots, stream=None) -> None:
 
 
 class Attention:
-    """The workspace of the attention calls on one GPU (pc_attn); calls on one
-    handle run one after another, so use one per stream."""
+    """The workspace of the attention calls on one GPU (pc_attn).
+
+    Calls on one handle run one after another: a call on another stream than
+    the last one's first makes its stream wait for that one, so programs that
+    use several streams want a handle for each.  (A stream given as a bare
+    handle has to live until then.)  A graph's replays are not seen here: they
+    and other calls on the handle are the caller's to keep apart.
+    """
 
     def __init__(self, device: int = 0):
         h = C.c_void_p()
         _check(_entry().pc_attn_create(device, C.byref(h)))
         self._h, self.device = h, device
+        self._last = self._last_given = None  # the last call's stream, and the object it was given as
+
+    def _on(self, stream):
+        """The stream of a call, behind the calls before it."""
+        st = _stream(self.device, stream)
+        if st != self._last:
+            self._follow(st, stream)
+        return st
+
+    def _follow(self, st, stream):
+        import torch
+
+        def of(handle):
+            return torch.cuda.ExternalStream(handle, device=self.device) if handle else torch.cuda.default_stream(self.device)
+
+        def capturing(s):
+            with torch.cuda.stream(s):
+                return torch.cuda.is_current_stream_capturing()
+
+        new = of(st)
+        if capturing(new):
+            return  # only records; it cannot wait for what is outside its graph
+        if self._last is not None:
+            old = of(self._last)
+            if not capturing(old):
+                new.wait_stream(old)
+        self._last, self._last_given = st, stream
 
     def _call(self, q, cu_new, sinks, window, scale, kv_heads, out, stream):
         """(bytes of the pc_attn_call, out, requests)"""
@@ -239,7 +272,7 @@ class Attention:
         if page_table.shape != (B, width):
             raise ValueError(f"page_table: [{B}, max_pages] expected")
         _check(_L.pc_attn_paged(self._h, c, p, _ints(page_table, "page_table", dev, B * width, _i32), width,
-                                _ints(kv_len, "kv_len", dev, B, _i32), _stream(dev, stream)))
+                                _ints(kv_len, "kv_len", dev, B, _i32), self._on(stream)))
         return out
 
     def packed(self, q, k, v, cu_new, *, sinks=None, window: int = 0, scale=None, out=None, stream=None):
@@ -255,7 +288,7 @@ class Attention:
         if shape != vshape or k.dtype is not q.dtype or v.dtype is not q.dtype or shape[0] != T or shape[2] != D:
             raise ValueError("k and v: [rows, kv_heads, head_dim] of q's rows, head_dim and type expected")
         _check(_L.pc_attn_packed(self._h, c, k.data_ptr(), _two_bytes(ks[0], ks[1]), v.data_ptr(),
-                                 _two_bytes(vs[0], vs[1]), _stream(dev, stream)))
+                                 _two_bytes(vs[0], vs[1]), self._on(stream)))
         return out
 
     def check(self, stream=None):

@@ -643,6 +643,40 @@ def test_side_stream_and_graph():
         assert torch.equal(out, eager)
 
 
+def test_one_handle_on_two_streams():
+    """Calls on one handle from stream to stream follow one another: they share
+    its workspace."""
+    torch = _torch()
+    from picchio_b200 import Attention
+    att = Attention()
+    sets = [make_paged(r, 16, 16, 2, 64, d, s) for s, (r, d) in enumerate(
+        (([(9000, 1), (3000, 1)], "bf16"), ([(5000, 300), (900, 33)], "f16"), ([(7000, 2)], "f32"), ([(4000, 4)] * 5, "bf16")))]
+    want = [handle().paged(*t) for t in sets]
+    streams = [torch.cuda.Stream() for _ in range(3)] + [torch.cuda.current_stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(24):
+        s = streams[i % 4]
+        if i % 3:
+            got.append(att.paged(*sets[i % 4], stream=s if i % 2 else s.cuda_stream))
+        else:
+            with torch.cuda.stream(s):
+                got.append(att.paged(*sets[i % 4]))
+    torch.cuda.synchronize()
+    att.check()
+    for i, g in enumerate(got):
+        assert torch.equal(g.view(torch.uint8), want[i % 4].view(torch.uint8)), i
+    # a graph of a call, beside calls on other streams before and after it
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = att.paged(*sets[0])
+    again = att.paged(*sets[1])
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0]) and torch.equal(again, want[1])
+
+
 # ---- tables and store ---------------------------------------------------------
 
 
