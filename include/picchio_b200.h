@@ -345,7 +345,8 @@ typedef struct {
  * Request b is not served if its new length exceeds max_pages pages, or if
  * it needs pages and the needs of requests 0 .. b exceed the free ones, or if
  * it adds positions and those of requests 0 .. b exceed n_tokens (sums over
- * all requests that fit their table).  free_cap and n_tokens are at most 2^28.
+ * all requests that fit their table).  free_cap and n_tokens are at most 2^28;
+ * n_requests may be 0 (the arrays with an element a request are not read then).
  * The inputs other than page_table and free_pages are not written: a call
  * repeated with the same inputs gives the same outputs, and the next step's
  * inputs are kv_end and n_free_out.  kv_end and n_free_out must not overlap the

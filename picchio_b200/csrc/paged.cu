@@ -164,9 +164,10 @@ pc_status run_attention(pc_attn *a, const AttnOp &o, int dtype, cudaStream_t st)
 extern "C" {
 
 pc_status pc_kv_tables(int device, const pc_kv_step *s, void *stream) {
-    if (!s || s->n_requests < 1 || s->max_pages < 1 || s->n_tokens < 0 || s->free_cap < 0 || !s->kv_len_dev ||
-        !s->new_len_dev || !s->n_free_dev || !s->page_table_dev || !s->kv_end_dev || !s->cu_new_dev ||
-        !s->served_dev || !s->n_free_out_dev || (s->free_cap > 0 && !s->free_pages_dev) ||
+    if (!s || s->n_requests < 0 || s->max_pages < 1 || s->n_tokens < 0 || s->free_cap < 0 || !s->n_free_dev ||
+        !s->cu_new_dev || !s->n_free_out_dev || (s->free_cap > 0 && !s->free_pages_dev) ||
+        (s->n_requests > 0 &&
+         (!s->kv_len_dev || !s->new_len_dev || !s->page_table_dev || !s->kv_end_dev || !s->served_dev)) ||
         (s->n_tokens > 0 && (!s->pos_dev || !s->slot_dev)))
         return fail(PC_ERR_INVALID_ARG, "bad pc_kv_tables arguments");
     if (s->page_size < 8 || s->page_size % 8 || s->page_size > (1 << 16))
@@ -174,7 +175,7 @@ pc_status pc_kv_tables(int device, const pc_kv_step *s, void *stream) {
     if (s->n_requests > (1 << 20) || s->n_tokens > (1 << 28) || s->free_cap > (1 << 28) ||
         (int64_t)s->max_pages * s->page_size > INT_MAX / 2)
         return fail(PC_ERR_RANGE, "too many requests, tokens, free pages or positions");
-    if (s->kv_end_dev == s->kv_len_dev || s->n_free_out_dev == s->n_free_dev)
+    if ((s->n_requests > 0 && s->kv_end_dev == s->kv_len_dev) || s->n_free_out_dev == s->n_free_dev)
         return fail(PC_ERR_INVALID_ARG, "kv_end and n_free_out must not overlap the inputs");
     OnDevice on(device);
     PC_CU(on.e);

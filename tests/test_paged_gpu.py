@@ -747,6 +747,17 @@ def test_tables_decode_and_pages():
     run_tables([5, 5], [0, -1], 2, 8, 0, 4)
 
 
+def test_tables_without_requests():
+    """A step with no request: no rows, the free pages as they were."""
+    torch = _torch()
+    from picchio_b200 import kv_tables
+    ti = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for n in (0, 5, 3000):
+        t = kv_tables(ti(), ti(), ti().view(0, 4), ti(7, 3, 9), ti(2), page_size=16, n_tokens=n)
+        assert t.cu_new.tolist() == [0] and t.n_free.tolist() == [2] and t.kv_len.numel() == t.served.numel() == 0
+        assert t.positions.tolist() == [-1] * n and t.slots.tolist() == [-1] * n
+
+
 def test_tables_refusals_of_requests():
     run_tables([10, 60, 3, 64, 20], [7, 5, 0, 1, 100], 4, 16, 3, 200)      # past the table's width
     run_tables([16, 16, 16, 5, 16], [1, 40, 1, 1, 1], 8, 16, 3, 100)       # pages run out at the second
