@@ -11,6 +11,7 @@ device unless ``stream`` is given, and waits for nothing.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 from typing import NamedTuple
 
@@ -104,6 +105,11 @@ def _made(t, stream):
     return t
 
 
+def _int(x):
+    """x as a C int; what one does not hold is out of every range the library takes."""
+    return min(max(int(x), -1), 0x7fffffff)
+
+
 def _type(t, name):
     d = _dt.get(t.dtype)
     if d is None:
@@ -150,8 +156,8 @@ def kv_tables(kv_len, new_len, page_table, free_pages, n_free, *, page_size: int
     """
     L = _entry()
     dev, B, width = kv_len.get_device(), kv_len.numel(), page_table.shape[-1]
-    if dev < 0 or page_table.shape != (B, width) or n_tokens < 0:
-        raise ValueError("kv_len on a CUDA device, page_table [requests, max_pages] and n_tokens >= 0 expected")
+    if dev < 0 or page_table.shape != (B, width) or not 0 <= n_tokens <= 1 << 28:
+        raise ValueError("kv_len on a CUDA device, page_table [requests, max_pages] and n_tokens from 0 to 2^28 expected")
     cap = free_pages.numel()
     if not (kv_len.dtype is new_len.dtype is page_table.dtype is free_pages.dtype is n_free.dtype is _i32
             and new_len.get_device() == page_table.get_device() == free_pages.get_device() == n_free.get_device() == dev
@@ -164,7 +170,7 @@ def kv_tables(kv_len, new_len, page_table, free_pages, n_free, *, page_size: int
     base = buf.data_ptr()
     end = base + 4 * (B + 1)
     served = end + 4 * B
-    s = _step_bytes.pack(B, width, page_size, n_tokens, cap, kv_len.data_ptr(), new_len.data_ptr(), n_free.data_ptr(),
+    s = _step_bytes.pack(B, width, _int(page_size), n_tokens, cap, kv_len.data_ptr(), new_len.data_ptr(), n_free.data_ptr(),
                          page_table.data_ptr(), free_pages.data_ptr(), end, base, served, served + 4 * B,
                          served + 4 * B + 4, slots.data_ptr())
     _check(L.pc_kv_tables(dev, s, _stream(dev, stream)))
@@ -250,8 +256,8 @@ class Attention:
             sp = sinks.data_ptr()
         n = cu_new.numel()
         return _call_bytes.pack(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], _type(q, "q"), H, kv_heads, D, T,
-                                n - 1, _ints(cu_new, "cu_new", dev, n, _i32), sp, min(int(window), 0x7fffffff),
-                                D ** -0.5 if scale is None else scale), out, n - 1
+                                n - 1, _ints(cu_new, "cu_new", dev, n, _i32), sp, _int(window),
+                                D ** -0.5 if scale is None else scale if -3e38 < scale < 3e38 else math.inf), out, n - 1
 
     def paged(self, q, k_pages, v_pages, page_table, cu_new, kv_len, *, sinks=None, window: int = 0, scale=None,
               out=None, stream=None):

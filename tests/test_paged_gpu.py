@@ -867,3 +867,24 @@ def test_attention_refusals():
         kv_store(kp, vp, q[:, :2], q[:, :2], torch.zeros(2, dtype=torch.int32, device="cuda"))
     empty = q[:0]
     assert a.paged(empty, kp, vp, table, ti(0, 0), kv).shape == (0, 4, 64)
+
+
+def test_numbers_out_of_every_range_are_refused():
+    """Numbers that a C int or float does not hold, and a step of more rows
+    than the tables count, by the library's own errors."""
+    torch = _torch()
+    from picchio_b200 import PicchioError, kv_tables
+    q, kp, vp, table, cu, kv = make_paged([(20, 2)], 16, 4, 2, 64, "bf16", 1)
+    ti = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for window in (-(1 << 40), -5):
+        with pytest.raises(PicchioError, match="PC_ERR_INVALID_ARG"):
+            handle().paged(q, kp, vp, table, cu, kv, window=window)
+    for scale in (1e300, -1e300, float("inf"), float("nan"), 0.0):
+        with pytest.raises(PicchioError, match="PC_ERR_INVALID_ARG"):
+            handle().paged(q, kp, vp, table, cu, kv, scale=scale)
+    for page in (1 << 40, -(1 << 40)):
+        with pytest.raises(PicchioError, match="PC_ERR_FORMAT"):
+            kv_tables(ti(1), ti(1), ti([1]).view(1, 1), ti(1, 2), ti(2), page_size=page, n_tokens=1)
+    for n in (-1, (1 << 28) + 1, 1 << 40):
+        with pytest.raises(ValueError):
+            kv_tables(ti(1), ti(1), ti([1]).view(1, 1), ti(1, 2), ti(2), page_size=16, n_tokens=n)
