@@ -13,11 +13,10 @@
 // rounded to the type, and what the rounding left has a product of its own: the
 // tensor pipe has room, and the error of bf16 outputs is that of their own
 // rounding (decode of 64 requests 1.97e-3 -> 1.66e-3 from the exact result; 109.5
-// -> 110.0 us, head size 128 184.4 -> 186.0).  (With
-// the rows as the M side, half of the products and of the exponentials were of
-// rows that did not exist: head size 128 211 us where it is 184 now, one token
-// 16 us where it is 14.)  The legacy products are far below their rate while
-// the tiles arrive.
+// -> 110.0 us, head size 128 184.4 -> 186.0).  (With the rows as the M side, half
+// of the products and of the exponentials were of rows that did not exist: head
+// size 128 211 us where it was 184, one token 16 us where it was 14.)  The legacy
+// products are far below their rate while the tiles arrive.
 //
 // A warp fetches its own tiles by TMA, the next one as soon as it is done with
 // one and across the ends of items, so the memory system does not see where
@@ -29,11 +28,15 @@
 //
 // Measured: one token each of 64 requests of 500-8000 positions, 64 query over
 // 8 KV heads of 64, bf16, pages of 16: 110 us, 5.4 TB/s (83 % of the measured
-// copy); 32 over 8 heads of 128, f16, pages of 32: 186 us, 6.4 TB/s (98 %).
+// copy; 114 with the launch of the many-row kernel behind it, which finds nothing
+// to do); 32 over 8 heads of 128, f16, pages of 32: 186 us, 6.4 TB/s (98 %; 189).
 // 64-wide heads read 128 bytes of each 1 KB row; with pages laid out heads
-// first they are 6 % faster.  One token over 4096 positions takes 14 us: 2.5 us
+// first they are 6 % faster.  One token over 4096 positions takes 15 us: 2.5 us
 // to find the shares, about 2 until the first tile is there, the rest its work,
-// the joins and their trips to L2.
+// the joins and their trips to L2.  What an item costs beside its keys counts as
+// 256 of them in the shares (128, 512: 64 requests 117, 111 us where it is 113, 300
+// tokens to 600 of 128-wide heads 128, 95 where it is 90, one token 14.1, 15.2
+// where it is 14.8).
 #include <algorithm>
 
 #include "attention_half.cuh"

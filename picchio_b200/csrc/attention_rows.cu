@@ -39,7 +39,7 @@
 // it or just above (a whole power of two from the old one), O and what is
 // written of the tile rescaled.  (First references of whole powers of two, so
 // that every move is one, round the largest weight, which is 1 otherwise: 16
-// prompts 2.35e-3 from the exact result instead of 2.11e-3.)  (Each item's first
+// prompts 2.35e-3 from the exact result instead of 2.11e-3.  Each item's first
 // tile searched whole: 16 prompts 341 us instead of 312.)
 //
 // A key that a row does not see has weight 0, but 0 x NaN is NaN: in tiles
@@ -50,14 +50,17 @@
 //
 // Bound by the row warps: a tile pair's products take 1024 tensor cycles, its
 // 32,768 exponentials 2048 cycles of the special-function units, and the row
-// warps need about 3000 with their waits, instruction fetch among them (loop
-// bodies of more than ~150 instructions, or more code inlined beside them, cost
-// more than they save: unrolling the weights' loop by two took 16 prompts from
-// 338 to 393 us); an item costs about 6000 more.  At head size 128 the two S
+// warps need about 3000: two of them a scheduler use 41 % of its issue slots, and
+// what lies between are the fixed latencies of dependent instructions (2.3 cycles
+// an instruction) and waits for TMEM loads (2.0); instruction fetch is 0.2 in this
+// form, and what made earlier ones slower (the weights' loop
+// unrolled by two: 16 prompts 338 -> 393 us).  An item costs about 6000 cycles more,
+// which the shares count as 256 keys (128, 384, 640: 16 prompts 340, 328, 360 us
+// where it is 311; a window of 128 or 40 chunks of 100 alike).  At head size 128 the two S
 // buffers leave each row tile waiting for its products (2000 of 4300 cycles a
 // tile; S in halves of 64 keys or the row tiles in turn: no better).  Measured:
-// 16 prompts of 100-2048 tokens, 64 query over 8 KV heads of 64, bf16: 309 us,
-// 516 TFLOP/s; four of 1500-4000 with a window of 128: 145 us, 1.5 TB/s; one of
+// 16 prompts of 100-2048 tokens, 64 query over 8 KV heads of 64, bf16: 311 us,
+// 513 TFLOP/s; four of 1500-4000 with a window of 128: 146 us, 1.5 TB/s; one of
 // 8191, 32 over 8 heads of 128, f16: 605 us, 910 TFLOP/s (cuBLAS bf16 1669).
 #include <algorithm>
 #include <climits>

@@ -3,8 +3,8 @@
 // bf16 ones whose strides no tensor map describes), head sizes up to 128.
 //
 // A thread block takes the items of its share (attention_plan.cuh).  R rows
-// (tokens x query heads of one KV head; 16, 32 or 64 of them, the least that
-// holds a request's) meet tiles of 64 keys: scores S = Q K^T from shared
+// (tokens x query heads of one KV head; 16, 32 or 64 of them, see simt_rows)
+// meet tiles of 64 keys: scores S = Q K^T from shared
 // memory (4 rows x 64/TX keys per thread: 8 16-byte loads for 64
 // multiply-adds), the running maximum and sum of each row across the TX
 // threads of its row group, then O += P V with O in registers (4 rows x HDP/TX
@@ -13,7 +13,10 @@
 // rows, by the waits of a tile's steps for one another.  Measured, fp32, 64
 // query over 8 KV heads of 64: prompts of 154, 259 and 287 tokens 80 us (the
 // multiply-adds alone 19 us, 25 with the masked ones), three tokens each of 15
-// requests of 173-1430 positions 46 us.
+// requests of 173-1430 positions 47 us.  What an item costs beside its keys counts
+// as 48 of them in the shares (24, 96, 160: the prompts 85, 83, 87 us, 64 single
+// tokens to 2000 174, 166, 167 where it is 161; four chunks of 500 over 1500 within
+// 1 %, the three tokens alike).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
